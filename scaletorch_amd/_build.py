@@ -35,6 +35,10 @@ ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 # canonicalisation hipcc inserts before every fmaxf on an MFMA result;
 # -amdgpu-mfma-vgpr-form keeps compiler-emitted MFMAs in VGPRs (their results
 # feed VALU) while the asm accumulate chains own the AGPRs (see mfma_acc).
+# No packed fp32 arithmetic (v_pk_add / mul / fma_f32, which -O3 forms from ordinary float
+# code): some of its forms have given wrong results on MI355X.  The host pass warns that it
+# does not know the feature; it has no effect there.
+HIP_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 FILE_FLAGS = {"flash_attn.hip": ["-fno-honor-nans", "-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 
@@ -96,7 +100,7 @@ def build(verbose: bool = False, jobs: int | None = None, force: bool = False, v
         obj = BUILD / (src.stem + ".o")
         objs.append(obj)
         if force or _stale(obj, [src, *headers, Path(__file__)]):
-            extra = FILE_FLAGS.get(src.name, []) + (variant_flags or {}).get(src.name, [])
+            extra = HIP_FLAGS + FILE_FLAGS.get(src.name, []) + (variant_flags or {}).get(src.name, [])
             jobs_list.append([hipcc, f"--offload-arch={ARCH}", *common_flags, *extra, "-c", str(src), "-o",
                               str(obj)])
     # host C++ (torch op registrations, hipBLASLt tuner): g++ against the PyTorch headers
