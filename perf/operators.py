@@ -307,7 +307,7 @@ def _run_adamw(s):
         a = s["lists"]
         ops.adamw_multi_(a["param"], a["grad"], a["exp_avg"], a["exp_avg_sq"], step=s["step"], lr=LR, betas=BETAS,
                          eps=ADAM_EPS, weight_decay=s["wd"], masters=a["master"], scales=a["scales"],
-                         clip_coef=s["clip"])
+                         clip_coef=s["clip"], scale_grads=s["grad"].dtype == torch.float32)  # fp32 ones stay clipped
         return _adamw_state(s)
     (b1, b2), t = BETAS, s["step"]
     p = s["param"] if s["master"] is None else s["master"]
