@@ -102,7 +102,8 @@ def main(argv=None) -> int:
     test = CharDataset(text[n_train:], dc["block_size"], full.chars)
     model = GPT(GPTConfig(vocab_size=full.vocab_size, block_size=dc["block_size"], **gc)).to(device)
     ddp = DataParallel(model, bucket_size=1 << 20, expose_grads=True)
-    opt = model.configure_optimizers(oc["weight_decay"], oc["learning_rate"], (0.9, 0.95), device.type)
+    opt = model.configure_optimizers(oc["weight_decay"], oc["learning_rate"], (0.9, 0.95), device.type,
+                                     state_dtype=oc.get("state_dtype"))
 
     start_epoch = 0
     snap = tc.get("snapshot_path")

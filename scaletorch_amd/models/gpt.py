@@ -325,11 +325,18 @@ class GPT(nn.Module):
         self.config.block_size = block_size
         self.transformer.wpe.weight = nn.Parameter(self.transformer.wpe.weight[:block_size])
 
-    def configure_optimizers(self, weight_decay, learning_rate, betas, device_type="cuda"):
+    def configure_optimizers(self, weight_decay, learning_rate, betas, device_type="cuda",
+                             state_dtype: str | None = None):
+        """``state_dtype`` "fp32" / "fp8": the framework's many-tensor AdamW with moments of that
+        type (optim.MultiTensorAdamW); None: ``torch.optim.AdamW``."""
         params = [p for p in self.parameters() if p.requires_grad]
         decay = [p for p in params if p.dim() >= 2]
         nodecay = [p for p in params if p.dim() < 2]
         groups = [{"params": decay, "weight_decay": weight_decay}, {"params": nodecay, "weight_decay": 0.0}]
+        if state_dtype is not None:
+            from ..optim import MultiTensorAdamW
+
+            return MultiTensorAdamW(groups, lr=learning_rate, betas=betas, state_dtype=state_dtype)
         fused = "fused" in inspect.signature(torch.optim.AdamW).parameters and device_type == "cuda"
         return torch.optim.AdamW(groups, lr=learning_rate, betas=betas, fused=fused)
 

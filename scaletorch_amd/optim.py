@@ -455,6 +455,106 @@ class ArenaLAMB(ArenaAdamW):
                 a.param_flat.copy_(master)
 
 
+class MultiTensorAdamW(torch.optim.Optimizer):
+    """AdamW over separate parameter tensors: every tensor of a step in one launch per 48 of them
+    (ops/adamw_multi.py), whatever the parameter groups.
+
+    ``state_dtype``: "fp32" moments, or "fp8": 2 bytes an element and 8 a block of 256 for both
+    moments instead of 8 an element.  bf16 / fp16 parameters get fp32 master weights.  The step
+    is for parameters outside the arenas (``GPT.configure_optimizers``); a model wrapped with
+    ``expose_grads`` works too.  State dicts load across the two state types."""
+
+    _MOMENTS = ("exp_avg", "exp_avg_sq", "scales", "master")
+
+    def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.0,
+                 state_dtype: str = "fp32"):
+        if state_dtype not in ("fp32", "fp8"):
+            raise ValueError(f"state_dtype must be fp32 or fp8, got {state_dtype!r}")
+        if lr < 0 or eps < 0 or weight_decay < 0 or not all(0.0 <= b < 1.0 for b in betas):
+            raise ValueError(f"invalid AdamW settings: lr {lr}, betas {betas}, eps {eps}, weight_decay {weight_decay}")
+        self.state_dtype = state_dtype
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+
+    def _init_state(self, p: torch.Tensor) -> dict:
+        from .ops.adamw_multi import adamw_blocks
+
+        dt = torch.float32 if self.state_dtype == "fp32" else torch.float8_e4m3fn
+        flat = dict(device=p.device, memory_format=torch.contiguous_format)
+        s = {"step": 0, "exp_avg": torch.zeros_like(p, dtype=dt, **flat),
+             "exp_avg_sq": torch.zeros_like(p, dtype=dt, **flat)}
+        if self.state_dtype == "fp8":
+            s["scales"] = torch.zeros(adamw_blocks(p.numel()), 2, device=p.device)
+        if p.dtype != torch.float32:
+            s["master"] = p.detach().float()
+        return s
+
+    @torch.no_grad()
+    def step(self, closure=None, clip_coef: torch.Tensor | None = None, scale_grads: bool = False):
+        """``clip_coef``: a device fp32 value that every gradient is multiplied by (no host sync);
+        ``scale_grads`` leaves the gradients so multiplied."""
+        from .ops.adamw_multi import adamw_multi_
+
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        # tensors of one learning rate, betas, eps, step and device go together; the decay is each tensor's own
+        calls: dict = {}
+        for g in self.param_groups:
+            for p in g["params"]:
+                if p.grad is None:
+                    continue
+                if p.grad.is_sparse:
+                    raise RuntimeError("MultiTensorAdamW does not support sparse gradients")
+                if not p.is_contiguous():
+                    raise RuntimeError("MultiTensorAdamW needs contiguous parameters")
+                if not p.grad.is_contiguous():
+                    p.grad = p.grad.contiguous()
+                s = self.state[p]
+                if not s:
+                    s.update(self._init_state(p))
+                key = (float(g["lr"]), tuple(g["betas"]), g["eps"], s["step"] + 1, p.device)
+                calls.setdefault(key, []).append((p, s, g["weight_decay"]))
+        for (lr, betas, eps, t, _), todo in calls.items():
+            states = [s for _, s, _ in todo]
+            adamw_multi_([p for p, _, _ in todo], [p.grad for p, _, _ in todo],
+                         [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states], step=t, lr=lr, betas=betas,
+                         eps=eps, weight_decay=[w for _, _, w in todo], masters=[s.get("master") for s in states],
+                         scales=[s.get("scales") for s in states], clip_coef=clip_coef,
+                         scale_grads=scale_grads)
+            for s in states:
+                s["step"] = t
+        return loss
+
+    @torch.no_grad()
+    def load_state_dict(self, state_dict) -> None:
+        """Loads either state type into this optimizer's own.  (The base class would cast every
+        state tensor to its parameter's dtype.)"""
+        from .ops.adamw_multi import adamw_pack8, adamw_unpack8
+
+        slim = {**state_dict, "state": {k: {"step": int(v["step"])} for k, v in state_dict["state"].items()}}
+        super().load_state_dict(slim)
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
+            got = state_dict["state"].get(i)
+            if not got:
+                continue
+            got = {k: got[k].detach().to(p.device).clone() for k in self._MOMENTS if got.get(k) is not None}
+            eight = got["exp_avg"].dtype == torch.float8_e4m3fn
+            if eight and self.state_dtype == "fp32":
+                got["exp_avg"], got["exp_avg_sq"] = adamw_unpack8(got["exp_avg"], got["exp_avg_sq"], got.pop("scales"))
+            elif not eight and self.state_dtype == "fp8":
+                got["exp_avg"], got["exp_avg_sq"], got["scales"] = adamw_pack8(got["exp_avg"].float(),
+                                                                               got["exp_avg_sq"].float())
+            elif not eight:
+                got["exp_avg"], got["exp_avg_sq"] = got["exp_avg"].float(), got["exp_avg_sq"].float()
+            if p.dtype == torch.float32:
+                got.pop("master", None)
+            elif "master" not in got:
+                got["master"] = p.detach().float()
+            self.state[p].update(got)
+
+
 def create_optimizer(dp_model, optimizer_type: str = "adamw", lr: float = 1e-3, weight_decay: float = 0.0,
                      betas=(0.9, 0.999), eps: float = 1e-8, use_fused_adam: bool = True, state_dtype: str = "fp32"):
     t = optimizer_type.lower()
