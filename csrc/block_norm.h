@@ -95,6 +95,58 @@ ST_DEVICE void st_lane(P* p, int lane, int lanes, int width, const float (&f)[8]
     if (col < width) st_row<VEC>(p + col, v);
   }
 }
+// The same still as loaded, so that a row can be requested ahead of its use.
+template <typename P>
+struct LaneRaw {
+  static constexpr int kWords = 8 * sizeof(P) / 4;
+  uint32_t w[kWords];
+};
+template <int VEC, typename P>
+ST_DEVICE void ld_raw(const P* p, int lane, int lanes, int width, LaneRaw<P>& r) {
+  if constexpr (VEC == 8) {
+    if (lane * 8 < width) {
+#pragma unroll
+      for (int i = 0; i < LaneRaw<P>::kWords / 4; ++i) {
+        const u32x4 v = reinterpret_cast<const u32x4*>(p + lane * 8)[i];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) r.w[4 * i + k] = v[k];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < LaneRaw<P>::kWords; ++i) r.w[i] = 0;
+    }
+  } else {
+    uint32_t e[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      const int col = c * lanes + lane;
+      e[c] = 0;
+      if (col < width) {
+        if constexpr (sizeof(P) == 4) e[c] = reinterpret_cast<const uint32_t*>(p)[col];
+        else e[c] = reinterpret_cast<const uint16_t*>(p)[col];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < LaneRaw<P>::kWords; ++i)
+      r.w[i] = sizeof(P) == 4 ? e[i] : e[(2 * i) & 7] | (e[(2 * i + 1) & 7] << 16);
+  }
+}
+template <typename P>
+ST_DEVICE void zero_raw(LaneRaw<P>& r) {
+#pragma unroll
+  for (int i = 0; i < LaneRaw<P>::kWords; ++i) r.w[i] = 0;
+}
+template <typename P>
+ST_DEVICE void widen(const LaneRaw<P>& r, float (&f)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if constexpr (sizeof(P) == 4) f[i] = __uint_as_float(r.w[i]);
+    else if constexpr (sizeof(P) == 2 && __is_same(P, bf16_t))
+      f[i] = __uint_as_float((i & 1) ? r.w[i >> 1] & 0xffff0000u : r.w[i >> 1] << 16);
+    else f[i] = __half2float(__ushort_as_half((unsigned short)(r.w[i >> 1] >> (16 * (i & 1)))));
+  }
+}
+
 // a weight, the row type T or fp32 (the same for a whole launch); columns behind the row: 0
 template <int VEC, typename T>
 ST_DEVICE void ld_weight(const void* w, int f32, int lane, int lanes, int width, float (&f)[8]) {
@@ -138,36 +190,31 @@ ST_DEVICE void ld_weights(const NormArgs& a, int lane, int lanes, float (&p1)[8]
   }
 }
 
-// Sums over a row's lanes: its wave's, or, where several waves share the row, through LDS.
+// Sums over a row's lanes: its wave's, or, where several waves share the row, through LDS.  The
+// sums take two buffers in turn, so that one barrier each is enough: who writes a buffer again has
+// passed the barrier of the sum between, which every wave reaches after reading this one.
 template <bool ONE>
-ST_DEVICE float2 row_sum2(float a, float b, float2* red) {
-  a = wave_sum(a);
-  b = wave_sum(b);
-  if constexpr (!ONE) {
-    const int waves = blockDim.x >> 6;
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = make_float2(a, b);
-    __syncthreads();
-    a = b = 0.f;
-    for (int i = 0; i < waves; ++i) {
-      a += red[i].x;
-      b += red[i].y;
+struct RowSum {
+  float2* red;  // [2][kNormWaves]
+  int turn = 0;
+  ST_DEVICE float2 two(float a, float b) {
+    a = wave_sum(a);
+    b = wave_sum(b);
+    if constexpr (!ONE) {
+      const int waves = blockDim.x >> 6;
+      float2* r = red + turn * kNormWaves;
+      turn ^= 1;
+      if ((threadIdx.x & 63) == 0) r[threadIdx.x >> 6] = make_float2(a, b);
+      __syncthreads();
+      a = b = 0.f;
+      for (int i = 0; i < waves; ++i) {
+        a += r[i].x;
+        b += r[i].y;
+      }
     }
-    __syncthreads();
+    return make_float2(a, b);
   }
-  return make_float2(a, b);
-}
-template <bool ONE>
-ST_DEVICE float row_sum(float a, float2* red) {
-  a = wave_sum(a);
-  if constexpr (!ONE) {
-    const int waves = blockDim.x >> 6;
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6].x = a;
-    __syncthreads();
-    a = 0.f;
-    for (int i = 0; i < waves; ++i) a += red[i].x;
-    __syncthreads();
-  }
-  return a;
-}
+  ST_DEVICE float one(float a) { return two(a, 0.f).x; }
+};
 
 }  // namespace st

@@ -8,9 +8,10 @@
 //   dw1 = scale gate A, db1 = scale gate B, dgate = scale (w1 A + b1 B)
 // so two column sums serve the norm after the block and its gate, whatever the gate.
 //
-// Where there is a norm after the block or a gate, s is recomputed from h and the residual in
-// fp32: that reads as much as s and h would, and s's rounding does not enter the gradients.  A
-// plain pre-norm keeps s alone (one stream less).
+// s is recomputed from h and the residual in fp32, so its rounding to 16 bits does not enter the
+// gradients (from the rounded s, dw2 had 1.5 times the error of one rounding).  Where a norm after
+// the block or a gate needs h anyway that reads no more; a plain pre-norm pays one stream for it,
+// and keeps s alone where the stream is fp32 or s is h itself.
 //
 // A workgroup walks rows with a fixed stride and keeps its column sums in registers; its partial
 // sums are added up by the second kernel in a fixed order (no atomics: results repeat bit for bit).
@@ -21,12 +22,19 @@ using namespace st;
 
 namespace {
 
-// GEN: a norm after the block or a gate (else s alone); BIAS: sums of dy / ds' are kept too
-template <typename T, typename S, int VEC, bool ONE, bool GEN, bool BIAS>
-__global__ __launch_bounds__(ONE ? 256 : 1024) void block_norm_bwd_kernel(NormArgs a) {
+constexpr int kStream = 0, kPlain = 1, kFull = 2;
+
+// MODE: from kStream s alone, from kPlain h and the residual, from kFull those with a norm after the
+// block or a gate; BIAS: sums of dy / ds' are kept too
+// MOST: the most threads of a workgroup, 256 where a wave has a row of its own; widths up to 4096 do
+// with 512, which leaves a lane enough registers for the next row's loads
+template <typename T, typename S, int VEC, int MOST, int MODE, bool BIAS>
+__global__ __launch_bounds__(MOST) void block_norm_bwd_kernel(NormArgs a) {
+  constexpr bool ONE = MOST == 256, GEN = MODE == kFull;
   constexpr int kArrays = (GEN ? 2 : 1) * (BIAS ? 2 : 1);
   constexpr int kA = 1, kDy = GEN ? 2 : 1, kB = 3;  // dy shat, [ds' hhat], [dy, [ds']]
-  __shared__ float2 red[kNormWaves];
+  __shared__ float2 red[2 * kNormWaves];
+  RowSum<ONE> sum{red};
   const int lanes = ONE ? 64 : (int)blockDim.x, t = ONE ? threadIdx.x & 63 : threadIdx.x;
   const int width = a.width;
   const float inv = 1.f / (float)width;
@@ -37,22 +45,39 @@ __global__ __launch_bounds__(ONE ? 256 : 1024) void block_norm_bwd_kernel(NormAr
   for (int k = 0; k < kArrays; ++k)
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[k][i] = 0.f;
+  // the wave's next row is requested before this one's sums: two rows of loads in flight
+  LaneRaw<T> nh, ndy;
+  LaneRaw<S> ns, nds;
+  float4 nst;
+  zero_raw(nh);
+  zero_raw(ns);
+  zero_raw(ndy);
+  zero_raw(nds);
+  auto request = [&](int64_t row) {
+    const int64_t base = row * width;
+    if constexpr (MODE != kStream) {
+      ld_raw<VEC>((const T*)a.h + base, t, lanes, width, nh);
+      if (a.res) ld_raw<VEC>((const S*)a.res + base, t, lanes, width, ns);
+    } else if (a.dy) {
+      ld_raw<VEC>((const S*)a.s + base, t, lanes, width, ns);
+    }
+    if (a.dy) ld_raw<VEC>((const T*)a.dy + base, t, lanes, width, ndy);
+    if (a.ds) ld_raw<VEC>((const S*)a.ds + base, t, lanes, width, nds);
+    nst = reinterpret_cast<const float4*>(a.stats)[row];
+  };
   const int64_t step = (int64_t)gridDim.x * (ONE ? 4 : 1);
-  for (int64_t row = ONE ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x; row < a.rows; row += step) {
+  int64_t row = ONE ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+  if (row < a.rows) request(row);
+  for (; row < a.rows; row += step) {
     const int64_t base = row * width;
     float x[8], s[8], dy[8], d[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = s[i] = dy[i] = d[i] = 0.f;
-    if constexpr (GEN) {
-      ld_lane<VEC>((const T*)a.h + base, t, lanes, width, x);
-      if (a.res) ld_lane<VEC>((const S*)a.res + base, t, lanes, width, s);
-    } else if (a.dy) {
-      ld_lane<VEC>((const S*)a.s + base, t, lanes, width, s);
-    }
-    if (a.dy) ld_lane<VEC>((const T*)a.dy + base, t, lanes, width, dy);
-    if (a.ds) ld_lane<VEC>((const S*)a.ds + base, t, lanes, width, d);
-    const float4 st = reinterpret_cast<const float4*>(a.stats)[row];
-    if constexpr (GEN) {  // x: hhat, s: the stream
+    widen(nh, x);
+    widen(ns, s);
+    widen(ndy, dy);
+    widen(nds, d);
+    const float4 st = nst;
+    if (row + step < a.rows) request(row + step);
+    if constexpr (MODE != kStream) {  // x: hhat, s: the stream
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         x[i] = (x[i] - st.x) * st.y;
@@ -71,7 +96,7 @@ __global__ __launch_bounds__(ONE ? 256 : 1024) void block_norm_bwd_kernel(NormAr
         p += dy[i] * s[i];
         q += dy[i];
       }
-      const float2 pq = row_sum2<ONE>(p, q, red);
+      const float2 pq = sum.two(p, q);
       const float cp = pq.x * inv, cq = a.layer ? pq.y * inv : 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) d[i] += st.w * (dy[i] - s[i] * cp - cq);
@@ -89,7 +114,7 @@ __global__ __launch_bounds__(ONE ? 256 : 1024) void block_norm_bwd_kernel(NormAr
       q += d[i];
     }
     if (GEN && a.w1) {
-      const float2 pq = row_sum2<ONE>(p, q, red);
+      const float2 pq = sum.two(p, q);
       const float cp = pq.x * inv, cq = a.layer ? pq.y * inv : 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) d[i] = st.y * (d[i] - x[i] * cp - cq);
@@ -116,16 +141,37 @@ __global__ __launch_bounds__(ONE ? 256 : 1024) void block_norm_bwd_kernel(NormAr
   }
 }
 
+// The workgroups' partial sums [blocks][arrays][width] in kParts parts of blocks each: a wave 64
+// columns, four waves a quarter of the part each, added in order.
+constexpr int kParts = 8;
+__global__ __launch_bounds__(256) void block_norm_colsum_kernel(const float* __restrict__ partial, int blocks,
+                                                                int arrays, int width, float* __restrict__ out) {
+  __shared__ float red[4][64];
+  const int q = threadIdx.x & 63, g = threadIdx.x >> 6, col = blockIdx.x * 64 + q;
+  const int64_t line = (int64_t)arrays * width, at = (int64_t)blockIdx.y * width + col;
+  const int per = (blocks + kParts - 1) / kParts, b1 = min(blocks, (int)(blockIdx.z + 1) * per);
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  if (col < width) {
+    int b = blockIdx.z * per + g;
+    for (; b + 12 < b1; b += 16)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) s[u] += partial[(b + 4 * u) * line + at];
+    for (; b < b1; b += 4) s[0] += partial[b * line + at];
+  }
+  red[g][q] = (s[0] + s[1]) + (s[2] + s[3]);
+  __syncthreads();
+  if (!g && col < width) out[blockIdx.z * line + at] = (red[0][q] + red[1][q]) + (red[2][q] + red[3][q]);
+}
+
 struct FinishArgs {
-  const float* partial;
-  int blocks, arrays, width;
-  int gen, bias;
+  const float* sums;  // [kParts][arrays][width]
+  int arrays, width;
+  int gen;
   const void *gate, *w1, *b1;
   int gate_n, w32;
   float scale;
   void *dgate, *dw1, *db1, *dw2, *db2;  // null: not wanted
   int tgate, tw1, tb1, tw2, tb2;        // whether they are fp32, else T
-  float* gate_part;                     // scalar gate: one sum a workgroup
 };
 
 template <typename T>
@@ -135,27 +181,18 @@ ST_DEVICE void put(void* p, int f32, int i, float v) {
   else st_row<1>((T*)p + i, f);
 }
 
-// 32 columns a workgroup, 32 groups of partial rows each summed in order, then the groups in order
+// One column a thread; with a scalar gate one workgroup takes all columns and adds up their gates.
 template <typename T>
 __global__ __launch_bounds__(1024) void block_norm_finish_kernel(FinishArgs f) {
-  __shared__ float red[4][32][33];
-  const int q = threadIdx.x & 31, g = threadIdx.x >> 5, col = blockIdx.x * 32 + q;
-  float s[4] = {0.f, 0.f, 0.f, 0.f};
-  if (col < f.width)
-    for (int b = g; b < f.blocks; b += 32)
+  __shared__ float red[16];
+  float total = 0.f;
+  for (int col = blockIdx.x * blockDim.x + threadIdx.x; col < f.width; col += gridDim.x * blockDim.x) {
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int b = 0; b < kParts; ++b)
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        if (k < f.arrays) s[k] += f.partial[((int64_t)b * f.arrays + k) * f.width + col];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) red[k][g][q] = s[k];
-  __syncthreads();
-  if (g) return;
-  for (int k = 0; k < 4; ++k) {
-    s[k] = red[k][0][q];
-    for (int i = 1; i < 32; ++i) s[k] += red[k][i][q];
-  }
-  float dg = 0.f;
-  if (col < f.width) {
+        if (k < f.arrays) s[k] += f.sums[((int64_t)b * f.arrays + k) * f.width + col];
     const float A = s[1], dyb = s[f.gen ? 2 : 1], B = s[3];
     if (f.dw2) put<T>(f.dw2, f.tw2, col, s[0]);
     if (f.db2) put<T>(f.db2, f.tb2, col, dyb);
@@ -164,38 +201,39 @@ __global__ __launch_bounds__(1024) void block_norm_finish_kernel(FinishArgs f) {
       const float k = f.scale * (f.gate_n ? ld_one<T>(f.gate, f.w32, f.gate_n > 1 ? col : 0) : 1.f);
       if (f.dw1) put<T>(f.dw1, f.tw1, col, k * A);
       if (f.db1) put<T>(f.db1, f.tb1, col, k * B);
-      dg = f.scale * (w * A + (f.b1 ? b * B : 0.f));
+      const float dg = f.scale * (w * A + (f.b1 ? b * B : 0.f));
       if (f.dgate && f.gate_n > 1) put<T>(f.dgate, f.tgate, col, dg);
+      total += dg;
     }
   }
-  if (f.gate_part) {
-    for (int o = 16; o > 0; o >>= 1) dg += __shfl_xor(dg, o, 32);
-    if (q == 0) f.gate_part[blockIdx.x] = dg;
+  if (f.gate_n != 1 || !f.dgate) return;
+  total = wave_sum(total);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = total;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 16; ++i) total += red[i];
+    put<T>(f.dgate, f.tgate, 0, total);
   }
 }
 
-template <typename T>
-__global__ __launch_bounds__(64) void block_norm_gate_kernel(const float* __restrict__ part, int n, void* dgate,
-                                                             int f32) {
-  float s = 0.f;
-  for (int i = threadIdx.x; i < n; i += 64) s += part[i];
-  s = wave_sum(s);
-  if (threadIdx.x == 0) put<T>(dgate, f32, 0, s);
-}
-
-template <typename T, typename S, int VEC, bool GEN, bool BIAS>
+template <typename T, typename S, int VEC, int MODE, bool BIAS>
 int launch(const NormArgs& a, int blocks, hipStream_t st) {
   const int waves = (a.width + 511) / 512;
   if (waves == 1)
-    block_norm_bwd_kernel<T, S, VEC, true, GEN, BIAS><<<(unsigned)blocks, 256, 0, st>>>(a);
+    block_norm_bwd_kernel<T, S, VEC, 256, MODE, BIAS><<<(unsigned)blocks, 256, 0, st>>>(a);
+  else if (waves <= 8)
+    block_norm_bwd_kernel<T, S, VEC, 512, MODE, BIAS><<<(unsigned)blocks, 64 * waves, 0, st>>>(a);
   else
-    block_norm_bwd_kernel<T, S, VEC, false, GEN, BIAS><<<(unsigned)blocks, 64 * waves, 0, st>>>(a);
+    block_norm_bwd_kernel<T, S, VEC, 1024, MODE, BIAS><<<(unsigned)blocks, 64 * waves, 0, st>>>(a);
   return (int)hipGetLastError();
 }
 template <typename T, typename S, int VEC>
 int launch(const NormArgs& a, int gen, int bias, int blocks, hipStream_t st) {
-  if (gen) return bias ? launch<T, S, VEC, true, true>(a, blocks, st) : launch<T, S, VEC, true, false>(a, blocks, st);
-  return bias ? launch<T, S, VEC, false, true>(a, blocks, st) : launch<T, S, VEC, false, false>(a, blocks, st);
+  if (gen) return bias ? launch<T, S, VEC, kFull, true>(a, blocks, st) : launch<T, S, VEC, kFull, false>(a, blocks, st);
+  if constexpr (sizeof(S) == 2)  // an fp32 stream keeps s
+    if (!a.s)
+      return bias ? launch<T, S, VEC, kPlain, true>(a, blocks, st) : launch<T, S, VEC, kPlain, false>(a, blocks, st);
+  return bias ? launch<T, S, VEC, kStream, true>(a, blocks, st) : launch<T, S, VEC, kStream, false>(a, blocks, st);
 }
 template <typename T, typename S>
 int launch(const NormArgs& a, int gen, int bias, int blocks, int vec, hipStream_t st) {
@@ -204,9 +242,9 @@ int launch(const NormArgs& a, int gen, int bias, int blocks, int vec, hipStream_
 
 template <typename T>
 int finish(const FinishArgs& f, hipStream_t st) {
-  const unsigned grid = (unsigned)((f.width + 31) / 32);
-  block_norm_finish_kernel<T><<<grid, 1024, 0, st>>>(f);
-  if (f.gate_part) block_norm_gate_kernel<T><<<1, 64, 0, st>>>(f.gate_part, (int)grid, f.dgate, f.tgate);
+  const bool scalar = f.gate_n == 1 && f.dgate;
+  const unsigned grid = scalar ? 1 : (unsigned)((f.width + 255) / 256);
+  block_norm_finish_kernel<T><<<grid, scalar ? 1024 : 256, 0, st>>>(f);
   return (int)hipGetLastError();
 }
 
@@ -217,12 +255,13 @@ extern "C" {
 // Workgroups of a backward, hence rows of its partial sums.
 int st_block_norm_bwd_blocks(int64_t rows, int width) {
   const int waves = (width + 511) / 512;
-  const int64_t need = waves == 1 ? (rows + 3) / 4 : rows, most = waves == 1 ? 1024 : 4096 / waves;
+  const int64_t need = waves == 1 ? (rows + 3) / 4 : rows, most = waves == 1 ? 512 : 2048 / waves;
   return (int)(need < most ? need : most);
 }
 
 int st_block_norm_bwd(const NormArgs* a, int gen, int bias, int blocks, int htype, int stype, int vec, hipStream_t st) {
   if (a->rows <= 0 || a->width <= 0 || a->width > kNormMaxWidth || (vec && a->width % 8) || blocks <= 0) return -2;
+  if (!gen && !a->s && (stype == kF32 || !a->h)) return -2;
   if (htype == kF32 && stype == kF32) return launch<float, float>(*a, gen, bias, blocks, vec, st);
   if (htype == kBF16 && stype == kBF16) return launch<bf16_t, bf16_t>(*a, gen, bias, blocks, vec, st);
   if (htype == kBF16 && stype == kF32) return launch<bf16_t, float>(*a, gen, bias, blocks, vec, st);
@@ -231,18 +270,23 @@ int st_block_norm_bwd(const NormArgs* a, int gen, int bias, int blocks, int htyp
   return -2;
 }
 
+// Floats of a backward's workspace (NormArgs::partial) for `arrays` column sums.
+int64_t st_block_norm_bwd_floats(int64_t rows, int width, int arrays) {
+  return (int64_t)(st_block_norm_bwd_blocks(rows, width) + kParts) * arrays * width;
+}
+
 // The gradients of the weights and the gate from a's partial sums.  out: dgate, dw1, db1, dw2, db2
-// (null: not wanted), out_f32: which of them are fp32 and not of h's type; gate_part: (width + 31) / 32
-// floats for a scalar gate.
+// (null: not wanted), out_f32: which of them are fp32 and not of h's type.
 int st_block_norm_finish(const NormArgs* a, int gen, int bias, int blocks, void* const* out, const int* out_f32,
-                         float* gate_part, int htype, hipStream_t st) {
+                         int htype, hipStream_t st) {
   FinishArgs f{};
-  f.partial = a->partial;
-  f.blocks = blocks;
   f.arrays = (gen ? 2 : 1) * (bias ? 2 : 1);
+  float* sums = a->partial + (int64_t)blocks * f.arrays * a->width;
+  const dim3 grid((unsigned)((a->width + 63) / 64), (unsigned)f.arrays, kParts);
+  block_norm_colsum_kernel<<<grid, 256, 0, st>>>(a->partial, blocks, f.arrays, a->width, sums);
+  f.sums = sums;
   f.width = a->width;
   f.gen = gen;
-  f.bias = bias;
   f.gate = a->gate;
   f.w1 = a->w1;
   f.b1 = bias ? a->b1 : nullptr;
@@ -251,7 +295,6 @@ int st_block_norm_finish(const NormArgs* a, int gen, int bias, int blocks, void*
   f.scale = a->scale;
   f.dgate = out[0]; f.dw1 = out[1]; f.db1 = out[2]; f.dw2 = out[3]; f.db2 = out[4];
   f.tgate = out_f32[0]; f.tw1 = out_f32[1]; f.tb1 = out_f32[2]; f.tw2 = out_f32[3]; f.tb2 = out_f32[4];
-  f.gate_part = a->gate_n == 1 && out[0] ? gate_part : nullptr;
   if (htype == kF32) return finish<float>(f, st);
   if (htype == kBF16) return finish<bf16_t>(f, st);
   return finish<__half>(f, st);

@@ -15,7 +15,8 @@ namespace {
 // ONE: a row is a wave's own, four rows a workgroup; else the workgroup's
 template <typename T, typename S, int VEC, bool ONE, bool BIAS>
 __global__ __launch_bounds__(ONE ? 256 : 1024) void block_norm_fwd_kernel(NormArgs a) {
-  __shared__ float2 red[kNormWaves];
+  __shared__ float2 red[2 * kNormWaves];
+  RowSum<ONE> sum{red};
   const int lanes = ONE ? 64 : (int)blockDim.x, t = ONE ? threadIdx.x & 63 : threadIdx.x;
   const int width = a.width;
   const float inv = 1.f / (float)width;
@@ -31,12 +32,12 @@ __global__ __launch_bounds__(ONE ? 256 : 1024) void block_norm_fwd_kernel(NormAr
       float s = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) s += in[i] ? x[i] : 0.f;
-      mean = row_sum<ONE>(s, red) * inv;
+      mean = sum.one(s) * inv;
     }
     float q = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) q += in[i] ? (x[i] - mean) * (x[i] - mean) : 0.f;
-    rstd = rsqrtf(row_sum<ONE>(q, red) * inv + a.eps);
+    rstd = rsqrtf(sum.one(q) * inv + a.eps);
   };
   const int64_t step = (int64_t)gridDim.x * (ONE ? 4 : 1);
   for (int64_t row = ONE ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x; row < a.rows; row += step) {

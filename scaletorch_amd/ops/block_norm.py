@@ -20,7 +20,6 @@ from . import _lib
 from .grad import accumulate_grad
 
 _TYPES = (torch.float32, torch.bfloat16, torch.float16)
-MAX_WIDTH = 8192
 
 
 def _normalize(x: torch.Tensor, layer: bool, eps: float) -> torch.Tensor:
@@ -52,14 +51,17 @@ def block_norm_ref(h, residual, layer, post_weight, post_bias, gate, scale, pre_
 
 
 class _BlockNormFn(torch.autograd.Function):
+    """For weights with ``main_grad``; without, csrc/block_norm_ops.cpp has the same in C++."""
+
     @staticmethod
     def forward(ctx, h, residual, gate, w1, b1, w2, b2, layer, scale, eps, write_s):
-        gen = w1 is not None or gate is not None
+        stream = h.dtype if residual is None else residual.dtype
+        alone = w1 is None and gate is None and (not write_s or stream == torch.float32)
         y, s, stats = _lib.ops().block_norm_fwd(h, residual, gate, w1, b1, w2, b2, layer, scale, eps, write_s, True)
         y = y if w2 is not None else None
         s = s if write_s else None
         # what the backward recomputes from (csrc/block_norm_bwd.hip): h and the residual, or s alone
-        rows = (h, residual, None) if gen else (None, None, s if write_s else h)
+        rows = (None, None, s if write_s else h) if alone else (h, residual, None)
         ctx.save_for_backward(*rows, stats, gate, w1, b1, w2, b2)
         ctx.meta = (layer, scale, eps, h.dtype, residual is not None, None if residual is None else residual.dtype)
         ctx.set_materialize_grads(False)
@@ -133,20 +135,18 @@ def block_norm(h: torch.Tensor, residual: torch.Tensor | None = None, *, kind: s
     value, or one a column, learned.  ``residual`` may be fp32 with 16-bit h: s has its type, y has
     h's.  Without ``pre_weight`` y is None.  Rows of at most 8192 columns on the GPU.  Weight
     gradients go to ``main_grad`` where a weight has one."""
-    _check(h, residual, kind, post_weight, post_bias, gate, pre_weight, pre_bias)
-    layer, scale = kind == "layer", float(scale)
     if not _lib.use_native(h) or h.numel() == 0:
-        return block_norm_ref(h, residual, layer, post_weight, post_bias, gate, scale, pre_weight, pre_bias, eps)
-    if h.shape[-1] > MAX_WIDTH:
-        raise ValueError(f"block_norm: rows of at most {MAX_WIDTH} columns, got {h.shape[-1]}")
+        _check(h, residual, kind, post_weight, post_bias, gate, pre_weight, pre_bias)
+        return block_norm_ref(h, residual, kind == "layer", post_weight, post_bias, gate, float(scale), pre_weight,
+                              pre_bias, eps)
+    if kind not in ("rms", "layer"):
+        raise ValueError(f"block_norm: kind must be 'rms' or 'layer', got {kind!r}")
+    weights = (gate, post_weight, post_bias, pre_weight, pre_bias)
+    if not any(getattr(w, "main_grad", None) is not None for w in weights):
+        return _lib.ops().block_norm.default(h, residual, *weights, kind == "layer", scale, eps)
+    # weights whose gradients live in an arena: the sums go there in fp32
+    _check(h, residual, kind, post_weight, post_bias, gate, pre_weight, pre_bias)
     same = residual is None and post_weight is None and gate is None and scale == 1.0  # s is h itself
-    if same and pre_weight is None:
-        return None, h
     hc, rc = h.contiguous(), None if residual is None else residual.contiguous()
-    args = [None if w is None else w.contiguous() for w in (gate, post_weight, post_bias, pre_weight, pre_bias)]
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (hc, rc, *args)):
-        y, s = _BlockNormFn.apply(hc, rc, *args, layer, scale, eps, not same)
-    else:
-        y, s, _ = _lib.ops().block_norm_fwd(hc, rc, *args, layer, scale, eps, not same, False)
-        y = y if pre_weight is not None else None
+    y, s = _BlockNormFn.apply(hc, rc, *weights, kind == "layer", float(scale), eps, not same)
     return y, h if same else s
