@@ -1,0 +1,120 @@
+// Matrix products with an epilogue (linear_act_*.hip): arguments and what the kernels share.
+//
+//   forward   z = x W^T + b,  y = act(z) + residual
+//   backward  dz = dy act'(z),  dx = dz W,  dW = dz^T x,  db = sum of dz over the rows
+//
+// One product C[m, n] = sum_k A(m, k) B(n, k) serves all three: an operand is stored with k
+// contiguous ([rows, k], kRow) or with its rows contiguous ([k, rows], kCol):
+//   y: x kRow, W kRow;   dx: dz kRow, W kCol;   dW: dz kCol, x kCol.
+#pragma once
+
+#include "linear_act_args.h"
+
+#include "common.h"
+#include <hip/hip_fp16.h>
+
+namespace st {
+
+typedef __bf16 bfx8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bfx4 __attribute__((ext_vector_type(4)));
+typedef _Float16 hx8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+// 16-bit types travel as raw bits; F16 says which they are
+ST_DEVICE float half_up(uint32_t h, bool f16) {
+  return f16 ? __half2float(__ushort_as_half((unsigned short)h)) : __uint_as_float(h << 16);
+}
+ST_DEVICE uint32_t half_down(float f, bool f16) {
+  return f16 ? (uint32_t)__half_as_ushort(__float2half(f)) : (uint32_t)f2bf(f);
+}
+ST_DEVICE u32x2 pack4(f32x4 v, bool f16) {
+  return u32x2{half_down(v[0], f16) | (half_down(v[1], f16) << 16), half_down(v[2], f16) | (half_down(v[3], f16) << 16)};
+}
+ST_DEVICE f32x4 unpack4(u32x2 p, bool f16) {
+  return f32x4{half_up(p[0] & 0xffffu, f16), half_up(p[0] >> 16, f16), half_up(p[1] & 0xffffu, f16),
+               half_up(p[1] >> 16, f16)};
+}
+
+// The activations, from one exponential and one reciprocal each (errors of some 2^-22 relative to
+// z: far below the rounding of a 16-bit result).  The normal distribution function takes the
+// rational approximation 7.1.26 of Abramowitz and Stegun, Handbook of Mathematical Functions:
+// erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2), t = 1 / (1 + p x), for x >= 0, off by 1.5e-7 at most;
+// negative x by symmetry.  So gelu is off by 1e-7 |z|.
+ST_DEVICE float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
+ST_DEVICE float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.f + fast_exp(-x)); }
+// Phi(z) and exp(-z^2 / 2)
+ST_DEVICE float normal_cdf(float z, float& e) {
+  const float x = __builtin_fabsf(z) * 0.70710678118654752f;
+  e = fast_exp(-x * x);
+  const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * x);
+  const float p = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+  const float c = 0.5f * p * e;  // Phi(-|z|)
+  return z < 0.f ? c : 1.f - c;
+}
+constexpr float kTanhA = 1.5957691216057308f, kTanhB = 0.044715f;  // 2 sqrt(2 / pi): (1 + tanh(a)) / 2 = sigmoid(2 a)
+
+ST_DEVICE float act_of(float z, int act) {
+  float e;
+  switch (act) {
+    case kRelu: return z > 0.f ? z : (z != z ? z : 0.f);
+    case kGelu: return z * normal_cdf(z, e);
+    case kGeluTanh: return z * sigmoid(kTanhA * (z + kTanhB * z * z * z));
+    case kSilu: return z * sigmoid(z);
+    default: return z;
+  }
+}
+ST_DEVICE float act_slope(float z, int act) {
+  switch (act) {
+    case kRelu: return z > 0.f ? 1.f : (z != z ? z : 0.f);
+    case kGelu: {
+      float e;
+      const float p = normal_cdf(z, e);
+      return p + z * e * 0.39894228040143268f;
+    }
+    case kGeluTanh: {
+      const float zz = __builtin_fminf(z * z, 1e6f);  // beyond: the slope is 0 or 1, and inf * 0 is kept out
+      const float p = sigmoid(kTanhA * z * (1.f + kTanhB * zz));
+      return p + z * p * (1.f - p) * kTanhA * (1.f + 3.f * kTanhB * zz);
+    }
+    case kSilu: {
+      const float p = sigmoid(z), q = z * (1.f - p);
+      return p + p * (p > 0.f ? q : 0.f);
+    }
+    default: return 1.f;
+  }
+}
+
+// The epilogue of four consecutive columns n .. n + 3 of row m (count of them inside the matrix;
+// vec: all four, with aligned rows).
+ST_DEVICE void epilogue4(const LinearEpi& e, int64_t m, int n, int count, bool vec, f32x4 v) {
+  const int64_t at = m * e.ldo + n;
+  if (vec && count >= 4) {
+    if (e.bias) v += unpack4(*reinterpret_cast<const u32x2*>((const uint16_t*)e.bias + n), e.f16);
+    if (e.z) *reinterpret_cast<u32x2*>((uint16_t*)e.z + at) = pack4(v, e.f16);
+    if (e.act) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = act_of(v[i], e.act);
+    }
+    if (e.res)
+      v += e.out_f32 ? *reinterpret_cast<const f32x4*>((const float*)e.res + at)
+                     : unpack4(*reinterpret_cast<const u32x2*>((const uint16_t*)e.res + at), e.f16);
+    if (e.beta) v += *reinterpret_cast<const f32x4*>((const float*)e.out + at);
+    if (e.out_f32) *reinterpret_cast<f32x4*>((float*)e.out + at) = v;
+    else *reinterpret_cast<u32x2*>((uint16_t*)e.out + at) = pack4(v, e.f16);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (i >= count) break;
+    float x = v[i];
+    if (e.bias) x += half_up(((const uint16_t*)e.bias)[n + i], e.f16);
+    if (e.z) ((uint16_t*)e.z)[at + i] = (uint16_t)half_down(x, e.f16);
+    x = act_of(x, e.act);
+    if (e.res) x += e.out_f32 ? ((const float*)e.res)[at + i] : half_up(((const uint16_t*)e.res)[at + i], e.f16);
+    if (e.beta) x += ((const float*)e.out)[at + i];
+    if (e.out_f32) ((float*)e.out)[at + i] = x;
+    else ((uint16_t*)e.out)[at + i] = (uint16_t)half_down(x, e.f16);
+  }
+}
+
+}  // namespace st

@@ -1,0 +1,277 @@
+// The product with its epilogue for every shape: BM x BN tiles, 2 x 2 waves, k in steps of 64.
+//
+// A step's operands go global -> registers (16-byte loads, or element by element where rows are not
+// aligned), issued a step ahead, then to one of two LDS images, from which the waves read their
+// MFMA fragments; one barrier a step.  kRow images are [rows][64 k], 16-byte chunk c of row r at
+// c ^ ((r >> 1) & 7); kCol images [64 k][rows] in 256-byte (64-column tiles: 128-byte) rows, read
+// with the transposing LDS read, chunk c of row k at c ^ swz(k).  Chunks behind an operand's end
+// are zeros.  Few tiles: k is split over workgroups, whose fp32 sums a second kernel adds up in
+// order before the epilogue.
+#include <algorithm>
+
+#include "linear_act.h"
+
+using namespace st;
+
+namespace {
+
+constexpr int BK = 64, NT = 256;
+typedef __attribute__((address_space(3))) char lds_t;
+
+template <bool F16>
+ST_DEVICE f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (F16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(hx8, a), __builtin_bit_cast(hx8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bfx8, a), __builtin_bit_cast(bfx8, b), c, 0, 0, 0);
+}
+
+// One operand of a tile: R rows (m or n), layout COL.
+template <int R, bool COL, bool VEC>
+struct Operand {
+  static constexpr int kChunks = R * BK / 8 / NT;  // 16-byte chunks a thread moves
+  static constexpr int kBytes = R * BK * 2;
+  const uint16_t* base;
+  int64_t ld;
+  int rows, K;
+  u32x4 reg[kChunks];
+
+  ST_DEVICE static int swz(int k) {  // kCol: spreads the 16 k rows of a transposed read over the banks
+    return R == 128 ? ((k & 3) << 2) | ((k >> 2) & 3) : ((k & 1) << 2) | ((k >> 1) & 3);
+  }
+  ST_DEVICE static int lds_at(int c) {  // byte of chunk c of the image
+    if constexpr (COL) {
+      constexpr int per = R / 8;
+      const int k = c / per, p = c % per;
+      return k * (R * 2) + 16 * (p ^ swz(k));
+    } else {
+      const int r = c >> 3, p = c & 7;
+      return r * 128 + 16 * (p ^ ((r >> 1) & 7));
+    }
+  }
+  ST_DEVICE void load(int k0, int kend) {
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      const int c = threadIdx.x + NT * i;
+      int r, k;
+      if constexpr (COL) {
+        k = k0 + c / (R / 8);
+        r = (c % (R / 8)) * 8;
+      } else {
+        r = c >> 3;
+        k = k0 + (c & 7) * 8;
+      }
+      const int64_t at = COL ? (int64_t)k * ld + r : (int64_t)r * ld + k;
+      u32x4 v = {0u, 0u, 0u, 0u};
+      if constexpr (VEC) {
+        if (r < rows && k < kend) v = *reinterpret_cast<const u32x4*>(base + at);
+      } else {
+        uint32_t e[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const bool in = COL ? (k < kend && r + j < rows) : (r < rows && k + j < kend);
+          e[j] = in ? base[at + j] : 0u;
+        }
+        v = u32x4{e[0] | (e[1] << 16), e[2] | (e[3] << 16), e[4] | (e[5] << 16), e[6] | (e[7] << 16)};
+      }
+      reg[i] = v;
+    }
+  }
+  ST_DEVICE void store(lds_t* img) const {
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i)
+      *reinterpret_cast<u32x4 __attribute__((address_space(3)))*>(img + lds_at(threadIdx.x + NT * i)) = reg[i];
+  }
+  // fragment of rows r0 .. r0 + 15, k 32 ks .. + 31: lane (g = lane / 16) holds k 8 g .. 8 g + 7 of row lane % 16
+  ST_DEVICE static u32x4 frag(const lds_t* img, int r0, int ks) {
+    const int lane = threadIdx.x & 63;
+    if constexpr (COL) {
+      const int g = lane >> 4, q = (lane >> 2) & 3, p = lane & 3;
+      u32x2 h[2];
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const int k = 32 * ks + 8 * g + 4 * hf + q, col = r0 + 4 * p;
+        const lds_t* at = img + k * (R * 2) + 16 * ((col >> 3) ^ swz(k)) + 2 * (col & 7);
+        h[hf] = __builtin_bit_cast(
+            u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((bfx4 __attribute__((address_space(3)))*)at));
+      }
+      return u32x4{h[0][0], h[0][1], h[1][0], h[1][1]};
+    } else {
+      const int r = r0 + (lane & 15), c = 4 * ks + (lane >> 4);
+      return *reinterpret_cast<const u32x4 __attribute__((address_space(3)))*>(img + r * 128 +
+                                                                              16 * (c ^ ((r >> 1) & 7)));
+    }
+  }
+};
+
+template <int BM, int BN, bool ACOL, bool BCOL, bool VEC, bool F16>
+__global__ __launch_bounds__(NT) void linear_tile_kernel(LinearArgs p) {
+  constexpr int WM = BM / 2, WN = BN / 2, FM = WM / 16, FN = WN / 16;
+  typedef Operand<BM, ACOL, VEC> OpA;
+  typedef Operand<BN, BCOL, VEC> OpB;
+  __shared__ __attribute__((aligned(16))) char smem_raw[2 * (OpA::kBytes + OpB::kBytes)];
+  lds_t* smem = (lds_t*)smem_raw;
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wid >> 1, wn = wid & 1;
+  const int nbn = (p.N + BN - 1) / BN, nbm = (p.M + BM - 1) / BM;
+  const int vb = xcd_remap((int)blockIdx.x, nbm * nbn);
+  // groups of 8 row blocks: the tiles an XCD holds at once share operand slices in its L2
+  const int per = 8 * nbn, grp = vb / per, in = vb % per, gsz = min(8, nbm - grp * 8);
+  const int m0 = (grp * 8 + in % gsz) * BM, n0 = (in / gsz) * BN;
+  // this workgroup's part of k, whole steps
+  const int steps = (p.K + BK - 1) / BK, split = (int)blockIdx.y;
+  const int s0 = (int)((int64_t)split * steps / p.splits), s1 = (int)((int64_t)(split + 1) * steps / p.splits);
+  OpA A;
+  OpB B;
+  A.base = (const uint16_t*)p.a + (ACOL ? (int64_t)m0 : (int64_t)m0 * p.lda);
+  B.base = (const uint16_t*)p.b + (BCOL ? (int64_t)n0 : (int64_t)n0 * p.ldb);
+  A.ld = p.lda;
+  B.ld = p.ldb;
+  A.rows = p.M - m0;
+  B.rows = p.N - n0;
+  f32x4 acc[FM][FN];
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  constexpr int kStage = OpA::kBytes + OpB::kBytes;
+  if (s0 < s1) {
+    A.load(s0 * BK, p.K);
+    B.load(s0 * BK, p.K);
+    A.store(smem);
+    B.store(smem + OpA::kBytes);
+  }
+  __syncthreads();
+  for (int s = s0; s < s1; ++s) {
+    const lds_t* cur = smem + ((s - s0) & 1) * kStage;
+    lds_t* nxt = smem + ((s - s0 + 1) & 1) * kStage;
+    if (s + 1 < s1) {
+      A.load((s + 1) * BK, p.K);
+      B.load((s + 1) * BK, p.K);
+    }
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      u32x4 fa[FM], fb[FN];
+#pragma unroll
+      for (int i = 0; i < FM; ++i) fa[i] = OpA::frag(cur, wm * WM + 16 * i, ks);
+#pragma unroll
+      for (int j = 0; j < FN; ++j) fb[j] = OpB::frag(cur + OpA::kBytes, wn * WN + 16 * j, ks);
+      // operands swapped: a lane holds 4 consecutive columns of one row
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = mfma<F16>(fb[j], fa[i], acc[i][j]);
+    }
+    if (s + 1 < s1) {
+      A.store(nxt);
+      B.store(nxt + OpA::kBytes);
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    const int m = m0 + wm * WM + 16 * i + (lane & 15);
+    if (m >= p.M) continue;
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+      const int n = n0 + wn * WN + 16 * j + 4 * (lane >> 4);
+      if (n >= p.N) continue;
+      if (p.splits > 1) {
+        float* w = p.ws + ((int64_t)split * p.M + m) * p.N + n;
+        if (VEC) {
+          *reinterpret_cast<f32x4*>(w) = acc[i][j];
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (n + r < p.N) w[r] = acc[i][j][r];
+        }
+      } else {
+        epilogue4(p.epi, m, n, p.N - n, VEC, acc[i][j]);
+      }
+    }
+  }
+}
+
+// The partial sums of the splits in order, then the epilogue; four columns a thread.
+__global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs p) {
+  const int quads = (p.N + 3) / 4;
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t m = id / quads;
+  const int n = (int)(id % quads) * 4;
+  if (m >= p.M) return;
+  const float* w = p.ws + m * p.N + n;
+  const int64_t step = (int64_t)p.M * p.N;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < p.splits; ++s, w += step) {
+    if (p.vec) {
+      v += *reinterpret_cast<const f32x4*>(w);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (n + r < p.N) v[r] += w[r];
+    }
+  }
+  epilogue4(p.epi, m, n, p.N - n, p.vec != 0, v);
+}
+
+template <int B, bool ACOL, bool BCOL>
+int launch(const LinearArgs& p, hipStream_t st) {
+  const int64_t tiles = (int64_t)((p.M + B - 1) / B) * ((p.N + B - 1) / B);
+  if (tiles >= (1LL << 31)) return -2;
+  const dim3 grid((unsigned)tiles, (unsigned)p.splits);
+  if (p.vec) {
+    if (p.epi.f16) linear_tile_kernel<B, B, ACOL, BCOL, true, true><<<grid, NT, 0, st>>>(p);
+    else linear_tile_kernel<B, B, ACOL, BCOL, true, false><<<grid, NT, 0, st>>>(p);
+  } else {
+    if (p.epi.f16) linear_tile_kernel<B, B, ACOL, BCOL, false, true><<<grid, NT, 0, st>>>(p);
+    else linear_tile_kernel<B, B, ACOL, BCOL, false, false><<<grid, NT, 0, st>>>(p);
+  }
+  if (p.splits > 1) {
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return (int)e;
+    const int64_t blocks = ((int64_t)p.M * ((p.N + 3) / 4) + 255) / 256;
+    if (blocks >= (1LL << 31)) return -2;
+    linear_join_kernel<<<(unsigned)blocks, 256, 0, st>>>(p);
+  }
+  return (int)hipGetLastError();
+}
+
+// Tile edge and splits of a product.
+struct Plan {
+  int tile, splits;
+};
+Plan plan(int M, int N, int K) {
+  auto tiles = [&](int b) { return (int64_t)((M + b - 1) / b) * ((N + b - 1) / b); };
+  const int steps = (K + BK - 1) / BK;
+  Plan r{tiles(128) >= 256 ? 128 : 64, 1};
+  const int64_t t = tiles(r.tile);
+  if (t < 512 && steps >= 8) r.splits = (int)std::min<int64_t>({(512 + t - 1) / t, steps / 4, 32});
+  return r;
+}
+
+}  // namespace
+
+extern "C" {
+
+// fp32 workspace elements of a product.
+int64_t st_linear_tile_ws(int M, int N, int K) {
+  const Plan r = plan(M, N, K);
+  return r.splits > 1 ? (int64_t)r.splits * M * N : 0;
+}
+
+// C = A B^T with the epilogue; acol / bcol: the operand's rows are contiguous.  ws: st_linear_tile_ws
+// floats.  -2: outside the kernel's.
+int st_linear_tile(LinearArgs* p, int acol, int bcol, hipStream_t st) {
+  if (p->M <= 0 || p->N <= 0 || p->K <= 0 || (acol && !bcol)) return -2;
+  const Plan r = plan(p->M, p->N, p->K);
+  p->splits = r.splits;
+  if (r.splits > 1 && !p->ws) return -2;
+  if (r.tile == 128) {
+    if (!bcol) return launch<128, false, false>(*p, st);
+    return acol ? launch<128, true, true>(*p, st) : launch<128, false, true>(*p, st);
+  }
+  if (!bcol) return launch<64, false, false>(*p, st);
+  return acol ? launch<64, true, true>(*p, st) : launch<64, false, true>(*p, st);
+}
+
+}  // extern "C"

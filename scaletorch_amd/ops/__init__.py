@@ -10,6 +10,7 @@ from .adamw_multi import adamw_blocks, adamw_multi_, adamw_pack8, adamw_unpack8
 from .attention import (apply_rope, apply_rope_ref, flash_attn, flash_attn_bwd, flash_attn_fwd,
                         qknorm_rope_attention, rope_attention, rope_tables, sdpa_ref)
 from .block_norm import block_norm
+from .linear_act import linear_act
 from .mlp import linear, swiglu, swiglu_ref
 from .norm import RMSNorm, add_rms_norm, rms_norm, rms_norm_ref
 from .xent import cross_entropy
@@ -19,5 +20,5 @@ __all__ = [
     "qknorm_rope_attention",
     "rope_tables", "sdpa_ref", "linear", "swiglu", "swiglu_ref", "RMSNorm", "add_rms_norm", "rms_norm",
     "rms_norm_ref", "cross_entropy", "adamw_multi_", "adamw_blocks", "adamw_pack8", "adamw_unpack8",
-    "block_norm",
+    "block_norm", "linear_act",
 ]

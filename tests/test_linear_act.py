@@ -1,0 +1,274 @@
+"""Linear with bias, activation and residual in the epilogue (ops/linear_act.py, csrc/linear_act_*.hip)
+against 64 bits.
+
+Tolerances, element by element.  A sum of k products in fp32 in any order is off by at most k 2^-24
+times the sum of the products' magnitudes.  The activations have slopes of at most 1.13 and are
+themselves computed to 2e-6 of |z| + 1e-7; an output is rounded once, by u = eps / 2 of its type.  In
+the backward z and dz are kept in x's type: dz is off by u |dz| + |dy| (C u |z| + 4e-6), C bounding
+the activation's second derivative (0.8 gelu and its tanh form 0.9, silu 0.5, relu 0), and dx, dW and
+db by the sums of those errors over the products' other factors.
+"""
+import pytest
+import torch
+
+from scaletorch_amd import ops
+from scaletorch_amd.models.gpt import GPT, GPTConfig
+from scaletorch_amd.ops.linear_act import linear_act_ref
+
+U32 = 2.0 ** -24
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+CURVE = {"none": 0.0, "relu": 0.0, "gelu": 0.8, "gelu_tanh": 0.9, "silu": 0.5}
+
+
+def _inputs(device, m, k, n, dtype, bias=True, residual=True, rdtype=None, seed=0, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+
+    def make(*shape, std=1.0, dt=dtype):
+        return (torch.randn(*shape, generator=g) * std).to(dt).to(device)
+
+    return dict(x=make(m, k, std=scale), w=make(n, k, std=k ** -0.5), b=make(n, std=0.5) if bias else None,
+                r=make(m, n, std=2.0, dt=rdtype or dtype) if residual else None, dy=make(m, n, dt=rdtype if residual and rdtype else dtype))
+
+
+def _run(c, act, f=ops.linear_act):
+    t = {k: None if c[k] is None else c[k].detach().clone().requires_grad_(True) for k in "xwbr"}
+    y = f(t["x"], t["w"], t["b"], t["r"], act)
+    some = [k for k in "xwbr" if t[k] is not None]
+    return y, dict(zip(some, torch.autograd.grad(y, [t[k] for k in some], c["dy"])))
+
+
+def _within(got, ref, bound, u, what):
+    got, ref, bound = got.detach().double().cpu(), ref.detach().double(), bound.detach()
+    tiny = 2.0 ** -24 if u == 2.0 ** -11 else 2.0 ** -60
+    over = (got - ref).abs() - (bound + u * (ref.abs() + bound) * 1.01 + tiny)
+    assert (over <= 0).all(), f"{what}: {over.max().item():.3g} past the bound"
+
+
+def _compare(c, act):
+    y, g = _run(c, act)
+    d = {k: None if v is None else v.double().cpu() for k, v in c.items()}
+    ry, rg = _run(d, act, lambda x, w, b, r, a: linear_act_ref(x, w, b, r, a))
+    u = torch.finfo(c["x"].dtype).eps / 2 if c["x"].dtype != torch.float32 else U32
+    x, w, dy = d["x"], d["w"], d["dy"]
+    (m, k), n = x.shape, w.shape[0]
+    z = x @ w.t() + (0 if d["b"] is None else d["b"])
+    ez = (k + 4) * U32 * (x.abs() @ w.abs().t() + (0 if d["b"] is None else d["b"].abs()))
+    ey = 1.13 * ez + 2e-6 * z.abs() + 1e-7 + 2 * U32 * (0 if d["r"] is None else d["r"].abs())
+    _within(y, ry, ey, torch.finfo(y.dtype).eps / 2, "y")
+    zz = z.clone().requires_grad_(True)
+    from scaletorch_amd.ops.linear_act import _act_ref
+    slope = torch.autograd.grad(_act_ref(zz, act).sum(), zz)[0]
+    dz = dy * slope
+    edz = u * dz.abs() + dy.abs() * (CURVE[act] * (u * z.abs() + ez) + 4e-6)
+    if act == "none":
+        edz = (u if c["dy"].dtype != c["x"].dtype else 0.0) * dz.abs()
+    if act == "relu":  # within z's error of zero the slope may be the other one
+        edz = edz + dy.abs() * (z.abs() <= ez).double()
+    if c["x"].dtype == torch.float16:
+        edz = edz + 2.0 ** -24
+    _within(g["x"], rg["x"], edz @ w.abs() + (n + 4) * U32 * ((dz.abs() + edz) @ w.abs()), u, "dx")
+    _within(g["w"], rg["w"], edz.t() @ x.abs() + (m + 4) * U32 * ((dz.abs() + edz).t() @ x.abs()), u, "dw")
+    if "b" in g:
+        _within(g["b"], rg["b"], edz.sum(0) + (m + 4) * U32 * dz.abs().sum(0), u, "db")
+    if "r" in g:
+        assert torch.equal(g["r"], c["dy"])
+    return y, g
+
+
+SHAPES = [(1, 8, 4), (1, 1, 1), (3, 33, 7), (16, 256, 128), (17, 1000, 264), (33, 72, 40), (64, 520, 1000), (65, 64, 64),
+          (65, 65, 65), (130, 1000, 200), (300, 136, 8), (257, 100, 333), (129, 24, 2048), (1000, 520, 264)]
+WIDE = [(512, 256, 512), (1025, 320, 776), (777, 1024, 264)]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,k,n", SHAPES + WIDE)
+def test_shapes(device, dtype, m, k, n):
+    _compare(_inputs(device, m, k, n, dtype), "gelu")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("act", ["none", "relu", "gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("residual", [None, "same", "fp32"])
+def test_each_part(device, act, bias, residual):
+    for k, (dtype, (m, kk, n)) in enumerate(((torch.bfloat16, (70, 96, 136)), (torch.float16, (9, 40, 24)),
+                                             (torch.bfloat16, (131, 77, 35)), (torch.float16, (515, 128, 264)))):
+        c = _inputs(device, m, kk, n, dtype, bias, residual is not None, torch.float32 if residual == "fp32" else None,
+                    seed=k, scale=2.0)
+        _compare(c, act)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("act", ["relu", "gelu", "gelu_tanh", "silu"])
+def test_activation_range(device, act):
+    """z from -60 to 60 by an identity weight, and zero, infinities and NaN."""
+    z = torch.cat([torch.linspace(-60, 60, 4096), torch.linspace(-6, 6, 4096), torch.tensor([0.0, -0.0])])
+    z = torch.nn.functional.pad(z, (0, 8200 - z.numel())).to(torch.bfloat16).view(-1, 8).to(device)
+    w = torch.eye(8, dtype=torch.bfloat16, device=device)
+    t = z.clone().requires_grad_(True)
+    y = ops.linear_act(t, w, residual=torch.zeros_like(z, dtype=torch.float32), activation=act)
+    (dx,) = torch.autograd.grad(y, t, torch.ones_like(y))
+    r = z.double().cpu().requires_grad_(True)
+    from scaletorch_amd.ops.linear_act import _act_ref
+    ry = _act_ref(r, act)
+    (rdx,) = torch.autograd.grad(ry, r, torch.ones_like(ry))
+    assert ((y.double().cpu() - ry).abs() <= 2e-6 * r.abs() + 1e-7).all()
+    assert ((dx.double().cpu() - rdx).abs() <= 2.0 ** -8 * rdx.abs() * 1.01 * 2 + 4e-6).all()
+    special = torch.tensor([[float("inf"), float("nan"), -float("inf"), 1e30, -1e30, 2.0, 3.0, 4.0]] * 3, device=device)
+    one = torch.ones(1, 1, device=device).bfloat16()
+    got = ops.linear_act(special.bfloat16().view(-1, 1), one, activation=act).float().view(3, 8)
+    assert got[0, 0] == float("inf") and got[0, 1].isnan() and got[0, 3] > 9e29 and got[0, 4] == 0 and (got[0, 5:] > 1.5).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_layouts(device):
+    """More dimensions, padded rows, shifted starts, columns of a wider tensor, a transposed weight, no rows."""
+    c = _inputs(device, 24, 72, 40, torch.bfloat16)
+    want, grads = _run(c, "silu")
+    y = ops.linear_act(c["x"].view(2, 3, 4, 72), c["w"], c["b"], c["r"].view(2, 3, 4, 40), "silu")
+    assert y.shape == (2, 3, 4, 40) and torch.equal(y.view(24, 40), want)
+    wide = torch.randn(24, 100, device=device).bfloat16()
+    wide[:, 5:77] = c["x"]
+    odd = torch.zeros(40 * 72 + 1, dtype=torch.bfloat16, device=device)[1:].view(40, 72).copy_(c["w"])
+    for x, w in ((wide[:, 5:77], c["w"]), (c["x"], odd), (c["x"], c["w"].t().contiguous().t()),
+                 (c["x"].t().contiguous().t(), c["w"])):
+        d = dict(c, x=x, w=w)
+        x, w = (v.detach().requires_grad_(True) for v in (x, w))
+        y = ops.linear_act(x, w, c["b"], c["r"], "silu")
+        # another order of the same fp32 sums, rounded once
+        assert (y.float() - want.float()).abs().max() <= 2.0 ** -7 * want.float().abs().max()
+        dx, dw = torch.autograd.grad(y, (x, w), c["dy"])
+        for a, b in ((dx, grads["x"]), (dw, grads["w"])):
+            assert (a.float() - b.float()).abs().max() <= 2.0 ** -6 * b.float().abs().max()
+    y = ops.linear_act(c["x"][:0], c["w"], c["b"], activation="gelu")
+    assert y.shape == (0, 40)
+    e = _inputs(device, 1, 72, 40, torch.bfloat16)
+    y = ops.linear_act(e["x"][0], e["w"], e["b"], e["r"][0], "relu")
+    assert y.shape == (40,)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_refusals(device):
+    x, w, b = (torch.zeros(s, dtype=torch.bfloat16, device=device) for s in ((4, 16), (8, 16), (8,)))
+    bad = [
+        ((x, w, b, None, "swish"), ValueError),
+        ((x, w.t(), None, None, "none"), ValueError),
+        ((x, w, b[:4], None, "none"), ValueError),
+        ((x, w, b, x, "none"), ValueError),
+        ((x, w.view(2, 4, 16), b, None, "none"), ValueError),
+        ((x, w.float(), None, None, "none"), TypeError),
+        ((x, w, b.half(), None, "none"), TypeError),
+        ((x, w, b, torch.zeros(4, 8, device=device, dtype=torch.float16), "none"), TypeError),
+        ((x.int(), w.int(), None, None, "none"), TypeError),
+    ]
+    for args, err in bad:
+        with pytest.raises(err):
+            ops.linear_act(*args)
+    if device == "cuda":
+        with pytest.raises(TypeError):
+            ops.linear_act(x.float(), w.float())
+        with pytest.raises((ValueError, RuntimeError)):
+            ops.linear_act(x, w.cpu())
+
+
+def test_gradients_against_differences():
+    g = torch.Generator().manual_seed(0)
+    x, w, b, r = (torch.randn(s, generator=g, dtype=torch.float64).requires_grad_(True) for s in ((3, 5), (4, 5), (4,), (3, 4)))
+    for act in ("gelu", "gelu_tanh", "silu"):
+        torch.autograd.gradcheck(lambda *a: ops.linear_act(*a, activation=act), (x, w, b, r))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+def test_gradients_against_differences_gpu(act):
+    """Central differences of the fp32 output along one direction of the bias."""
+    c = _inputs("cuda", 70, 96, 136, torch.bfloat16, rdtype=torch.float32)
+    _, g = _run(c, act)
+    e = 0.125  # an exact bf16 change of a bias that is kept in eighths
+    c["b"] = (c["b"].float() * 8).round().div(8).bfloat16()
+    _, g = _run(c, act)
+    f = lambda b: (ops.linear_act(c["x"], c["w"], b, c["r"], act).double() * c["dy"]).sum().item()  # noqa: E731
+    d = torch.sign(c["b"].float())
+    num = (f((c["b"].float() + e * d).bfloat16()) - f((c["b"].float() - e * d).bfloat16())) / (2 * e)
+    ana = (g["b"].double() * d).sum().item()
+    # 9520 terms, each with a third-derivative part of at most e^2 / 6 * 2 |dy| and roundings of z and dz of
+    # 2^-8: independent signs, so some 6 sqrt(9520) (0.006 + 0.008)
+    assert abs(num - ana) <= 6 * 9520 ** 0.5 * 0.014
+
+
+@pytest.mark.gpu
+def test_repeatable_streams_graphs_and_no_grad():
+    for shape in ((1000, 520, 264), (33, 72, 40), (2048, 512, 1280)):
+        c = _inputs("cuda", *shape, torch.bfloat16)
+        a, b = _run(c, "gelu"), _run(c, "gelu")
+        assert torch.equal(a[0], b[0]) and all(torch.equal(a[1][k], b[1][k]) for k in a[1])
+        with torch.no_grad():
+            assert torch.equal(ops.linear_act(c["x"], c["w"], c["b"], c["r"], "gelu"), a[0])
+        st = torch.cuda.Stream()
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            d = _run(c, "gelu")
+        torch.cuda.current_stream().wait_stream(st)
+        assert all(torch.equal(a[1][k], d[1][k]) for k in a[1])
+    leaf = {k: c[k].clone().requires_grad_(True) for k in "xwbr"}
+
+    def step():
+        y = ops.linear_act(leaf["x"], leaf["w"], leaf["b"], leaf["r"], "gelu")
+        return [y, *torch.autograd.grad(y, list(leaf.values()), c["dy"])]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):  # two graphs, each with its own workspaces
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = step()
+        graphs.append((graph, outs))
+    for k in range(3):
+        new = _inputs("cuda", 2048, 512, 1280, torch.bfloat16, seed=10 + k)
+        with torch.no_grad():
+            for n in "xwbr":
+                leaf[n].copy_(new[n])
+        for graph, _ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, outs in graphs:
+            for x, y in zip(outs, step()):
+                assert torch.equal(x, y)
+        torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+def test_main_grad_takes_the_sums():
+    c = _inputs("cuda", 512, 256, 512, torch.bfloat16)
+    t = {k: c[k].clone().requires_grad_(True) for k in "xwbr"}
+    for k in "wb":
+        t[k].main_grad = torch.full(t[k].shape, 2.0, device="cuda")
+    ops.linear_act(t["x"], t["w"], t["b"], t["r"], "gelu").backward(c["dy"])
+    _, g = _run(c, "gelu")
+    for k in "wb":
+        assert t[k].grad is None
+        # the plain gradient is the same sum rounded to bf16
+        assert ((t[k].main_grad - 2.0 - g[k].float()).abs() <= 2.0 ** -8 * 1.01 * g[k].float().abs() + 1e-3).all()
+    assert torch.equal(t["x"].grad, g["x"]) and torch.equal(t["r"].grad, g["r"])
+
+
+@pytest.mark.gpu
+def test_autocast_casts_as_linear_does():
+    x, w, b = (torch.randn(s, device="cuda") for s in ((40, 64), (32, 64), (32,)))
+    r = torch.randn(40, 32, device="cuda")
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        y = ops.linear_act(x, w, b, r, "gelu")
+    assert y.dtype == torch.float32
+    c = dict(x=x.detach().bfloat16(), w=w.detach().bfloat16(), b=b.bfloat16(), r=r, dy=torch.randn(40, 32, device="cuda"))
+    want, g = _run(c, "gelu")
+    assert torch.equal(y, want)
+    dx, dw = torch.autograd.grad(y, (x, w), c["dy"])
+    assert dx.dtype == torch.float32 and torch.equal(dx, g["x"].float()) and torch.equal(dw, g["w"].float())
