@@ -27,38 +27,52 @@ ST_DEVICE float half_up(uint32_t h, bool f16) {
 ST_DEVICE uint32_t half_down(float f, bool f16) {
   return f16 ? (uint32_t)__half_as_ushort(__float2half(f)) : (uint32_t)f2bf(f);
 }
-ST_DEVICE u32x2 pack4(f32x4 v, bool f16) {
-  return u32x2{half_down(v[0], f16) | (half_down(v[1], f16) << 16), half_down(v[2], f16) | (half_down(v[3], f16) << 16)};
+typedef __bf16 bfx2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+ST_DEVICE uint32_t pack2(float a, float b, bool f16) {
+  if (f16) return half_down(a, true) | (half_down(b, true) << 16);
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bfx2));  // one v_cvt_pk_bf16_f32
 }
+ST_DEVICE u32x2 pack4(f32x4 v, bool f16) { return u32x2{pack2(v[0], v[1], f16), pack2(v[2], v[3], f16)}; }
 ST_DEVICE f32x4 unpack4(u32x2 p, bool f16) {
   return f32x4{half_up(p[0] & 0xffffu, f16), half_up(p[0] >> 16, f16), half_up(p[1] & 0xffffu, f16),
                half_up(p[1] >> 16, f16)};
 }
 
 // The activations, from one exponential and one reciprocal each (errors of some 2^-22 relative to
-// z: far below the rounding of a 16-bit result).  The normal distribution function takes the
-// rational approximation 7.1.26 of Abramowitz and Stegun, Handbook of Mathematical Functions:
-// erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2), t = 1 / (1 + p x), for x >= 0, off by 1.5e-7 at most;
-// negative x by symmetry.  So gelu is off by 1e-7 |z|.
-ST_DEVICE float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
-ST_DEVICE float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.f + fast_exp(-x)); }
-// Phi(z) and exp(-z^2 / 2)
-ST_DEVICE float normal_cdf(float z, float& e) {
-  const float x = __builtin_fabsf(z) * 0.70710678118654752f;
-  e = fast_exp(-x * x);
-  const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * x);
-  const float p = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
-  const float c = 0.5f * p * e;  // Phi(-|z|)
-  return z < 0.f ? c : 1.f - c;
+// z: far below the rounding of a 16-bit result), in as few operations as can be: the epilogue of the
+// wide kernel runs them with nothing beside it.  The normal distribution function takes the rational
+// approximation 7.1.26 of Abramowitz and Stegun, Handbook of Mathematical Functions: erfc(x) =
+// (a1 t + ... + a5 t^5) exp(-x^2), t = 1 / (1 + p x), for x >= 0, off by 1.5e-7 at most, here with
+// x = |z| / sqrt(2) and erfc / 2 = Phi(-|z|), the factors folded into the constants.
+ST_DEVICE float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+ST_DEVICE float rcp(float x) { return __builtin_amdgcn_rcpf(x); }
+ST_DEVICE float sigmoid(float x) { return rcp(1.f + exp2_(x * -1.4426950408889634f)); }
+// Phi(-|z|) and e = exp(-z^2 / 2)
+ST_DEVICE float normal_tail(float z, float& e) {
+  const float a = __builtin_fabsf(z);
+  e = exp2_(z * (z * -0.72134752044448170f));
+  const float t = rcp(__builtin_fmaf(a, 0.23164190f, 1.f));
+  const float p = __builtin_fmaf(
+      t, __builtin_fmaf(t, __builtin_fmaf(t, __builtin_fmaf(t, 0.5307027145f, -0.7265760135f), 0.7107068705f), -0.142248368f),
+      0.127414796f);
+  return t * p * e;
 }
 constexpr float kTanhA = 1.5957691216057308f, kTanhB = 0.044715f;  // 2 sqrt(2 / pi): (1 + tanh(a)) / 2 = sigmoid(2 a)
+constexpr float kLog2e = 1.4426950408889634f;
 
 ST_DEVICE float act_of(float z, int act) {
   float e;
   switch (act) {
     case kRelu: return z > 0.f ? z : (z != z ? z : 0.f);
-    case kGelu: return z * normal_cdf(z, e);
-    case kGeluTanh: return z * sigmoid(kTanhA * (z + kTanhB * z * z * z));
+    case kGelu: {  // z Phi(z) = max(z, 0) - |z| Phi(-|z|); the fabs of an infinite z times a zero tail is kept out
+      const float c = normal_tail(z, e), a = __builtin_fminf(__builtin_fabsf(z), 1e30f);
+      return (z > 0.f ? z : (z != z ? z : 0.f)) - a * c;
+    }
+    case kGeluTanh: {
+      const float s = z * __builtin_fmaf(z * z, -kTanhA * kTanhB * kLog2e, -kTanhA * kLog2e);
+      return z * rcp(1.f + exp2_(s));
+    }
     case kSilu: return z * sigmoid(z);
     default: return z;
   }
@@ -68,8 +82,8 @@ ST_DEVICE float act_slope(float z, int act) {
     case kRelu: return z > 0.f ? 1.f : (z != z ? z : 0.f);
     case kGelu: {
       float e;
-      const float p = normal_cdf(z, e);
-      return p + z * e * 0.39894228040143268f;
+      const float c = normal_tail(z, e);
+      return (z < 0.f ? c : 1.f - c) + z * e * 0.39894228040143268f;
     }
     case kGeluTanh: {
       const float zz = __builtin_fminf(z * z, 1e6f);  // beyond: the slope is 0 or 1, and inf * 0 is kept out
@@ -98,7 +112,6 @@ ST_DEVICE void epilogue4(const LinearEpi& e, int64_t m, int n, int count, bool v
     if (e.res)
       v += e.out_f32 ? *reinterpret_cast<const f32x4*>((const float*)e.res + at)
                      : unpack4(*reinterpret_cast<const u32x2*>((const uint16_t*)e.res + at), e.f16);
-    if (e.beta) v += *reinterpret_cast<const f32x4*>((const float*)e.out + at);
     if (e.out_f32) *reinterpret_cast<f32x4*>((float*)e.out + at) = v;
     else *reinterpret_cast<u32x2*>((uint16_t*)e.out + at) = pack4(v, e.f16);
     return;
@@ -111,7 +124,6 @@ ST_DEVICE void epilogue4(const LinearEpi& e, int64_t m, int n, int count, bool v
     if (e.z) ((uint16_t*)e.z)[at + i] = (uint16_t)half_down(x, e.f16);
     x = act_of(x, e.act);
     if (e.res) x += e.out_f32 ? ((const float*)e.res)[at + i] : half_up(((const uint16_t*)e.res)[at + i], e.f16);
-    if (e.beta) x += ((const float*)e.out)[at + i];
     if (e.out_f32) ((float*)e.out)[at + i] = x;
     else ((uint16_t*)e.out)[at + i] = (uint16_t)half_down(x, e.f16);
   }

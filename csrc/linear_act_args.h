@@ -16,7 +16,6 @@ struct LinearEpi {
   int64_t ldo;
   int act;
   int out_f32;
-  int beta;          // add to what out holds (fp32)
   int f16;           // the 16-bit type is fp16, else bf16
 };
 

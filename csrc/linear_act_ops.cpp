@@ -14,7 +14,11 @@ using st::LinearArgs;
 extern "C" {
 int64_t st_linear_tile_ws(int M, int N, int K);
 int st_linear_tile(LinearArgs* p, int acol, int bcol, hipStream_t st);
+double st_linear_tile_us(int M, int N, int K);
 int st_linear_rows(const LinearArgs* p, hipStream_t st);
+int64_t st_linear_wide_ws(const LinearArgs* p);
+double st_linear_wide_us(const LinearArgs* p, int acol, int bcol);
+int st_linear_wide(const LinearArgs* p, int acol, int bcol, hipStream_t st);
 int st_linear_dz_runs(int64_t rows, int width);
 int st_linear_dz(const void* dy, int dy_f32, const void* z, void* dz, void* db, int db_f32, float* partial,
                  int64_t rows, int width, int act, int f16, int vec, hipStream_t st);
@@ -58,14 +62,17 @@ void product(const at::Tensor& A, bool acol, const at::Tensor& B, bool bcol, st:
   const int64_t ca = acol ? M : K, cb = bcol ? N : K;  // the contiguous dimension of each operand
   p.vec = vec && ca % 8 == 0 && cb % 8 == 0 && N % 4 == 0 && p.lda % 8 == 0 && p.ldb % 8 == 0 && aligned(A) && aligned(B);
   int rc = -2;
+  // few rows stream the weight; else whichever tiling is expected to be faster
   if (!acol && !bcol && M <= 64) rc = st_linear_rows(&p, stream());
   if (rc == -2) {
+    const double wide = st_linear_wide_us(&p, acol, bcol);
+    const bool use_wide = wide >= 0.0 && wide < st_linear_tile_us(p.M, p.N, p.K);
     at::Tensor ws;
-    if (const int64_t n = st_linear_tile_ws(p.M, p.N, p.K)) {
+    if (const int64_t n = use_wide ? st_linear_wide_ws(&p) : st_linear_tile_ws(p.M, p.N, p.K)) {
       ws = at::empty({n}, A.options().dtype(at::kFloat));
       p.ws = ws.data_ptr<float>();
     }
-    rc = st_linear_tile(&p, acol, bcol, stream());
+    rc = use_wide ? st_linear_wide(&p, acol, bcol, stream()) : st_linear_tile(&p, acol, bcol, stream());
   }
   TORCH_CHECK(rc == 0, "st_amd::linear_act launch failed with code ", rc);
 }

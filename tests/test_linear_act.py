@@ -77,7 +77,9 @@ def _compare(c, act):
 
 SHAPES = [(1, 8, 4), (1, 1, 1), (3, 33, 7), (16, 256, 128), (17, 1000, 264), (33, 72, 40), (64, 520, 1000), (65, 64, 64),
           (65, 65, 65), (130, 1000, 200), (300, 136, 8), (257, 100, 333), (129, 24, 2048), (1000, 520, 264)]
-WIDE = [(512, 256, 512), (1025, 320, 776), (777, 1024, 264)]
+# products that the 256 x 256 tiles take: whole and cut tiles, ragged edges, one step of k, several rounds
+WIDE = [(512, 256, 512), (1025, 320, 776), (777, 1024, 264), (4096, 512, 4104)]
+LARGE = [(2056, 2048, 2568), (8200, 64, 8192), (16448, 1280, 1288), (300, 8192, 1024)]
 
 
 @pytest.mark.parametrize("device", DEVICES)
@@ -85,6 +87,27 @@ WIDE = [(512, 256, 512), (1025, 320, 776), (777, 1024, 264)]
 @pytest.mark.parametrize("m,k,n", SHAPES + WIDE)
 def test_shapes(device, dtype, m, k, n):
     _compare(_inputs(device, m, k, n, dtype), "gelu")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act,residual,rdtype,dtype", [("gelu", True, torch.float32, torch.bfloat16), ("none", True, None, torch.float16),
+                                                       ("silu", True, None, torch.bfloat16), ("gelu_tanh", False, None, torch.bfloat16)])
+@pytest.mark.parametrize("m,k,n", LARGE)
+def test_large(m, k, n, act, residual, rdtype, dtype):
+    """Against fp32 products on the GPU (the library's, checked at 64 bits where that is quick), whole tensors."""
+    c = _inputs("cuda", m, k, n, dtype, True, residual, rdtype, seed=m)
+    y, g = _run(c, act)
+    d = {k: None if v is None else v.double() for k, v in c.items()}
+    ry, rg = _run(d, act, lambda x, w, b, r, a: linear_act_ref(x, w, b, r, a))
+    u = torch.finfo(dtype).eps / 2
+    for got, ref, uu in ((y, ry, torch.finfo(y.dtype).eps / 2), (g["x"], rg["x"], 3 * u), (g["w"], rg["w"], 3 * u), (g["b"], rg["b"], 3 * u)):
+        ref = ref.detach()
+        # the 2-norm: one rounding of y; z's, dz's and the result's own in the gradients; fp32 sums of up to
+        # 16448 terms of random signs, some sqrt(16448) 2^-24 of the result
+        err = ((got.detach().double() - ref).norm() / ref.norm()).item()
+        assert err <= uu + 2e-5, (got.shape, err)
+        # and no element further off than six times that of the largest
+        assert (got.detach().double() - ref).abs().max() <= 6 * (uu + 2e-5) * ref.abs().max()
 
 
 @pytest.mark.parametrize("device", DEVICES)
