@@ -52,6 +52,14 @@ class GPTConfig:
     use_optimized_routing: bool = True
     use_einsum_aggregation: bool = True
     expert_capacity_roundup: bool = True
+    # blocks through the fused operators (ops.linear_act, ops.block_norm): bias, GELU and residual in the
+    # products' epilogues, LayerNorm as one kernel
+    fused_ops: bool = False
+    # residual branches: a norm after the block too, a learned gate a channel (from `gate_init`), a scale
+    post_norm: bool = False
+    residual_gate: bool = False
+    gate_init: float = 1.0
+    residual_scale: float = 1.0
 
     def __post_init__(self) -> None:
         for n in ("block_size", "vocab_size", "n_layer", "n_head", "n_embd"):
@@ -93,6 +101,11 @@ class LayerNorm(nn.Module):
         return F.layer_norm(x, self.weight.shape, self.weight, self.bias, 1e-5)
 
 
+def _fusable(x: torch.Tensor) -> bool:
+    """Whether linear_act takes x: 16 bits (or made so by autocast) on the GPU, anything on the CPU."""
+    return not x.is_cuda or x.dtype in (torch.bfloat16, torch.float16) or torch.is_autocast_enabled("cuda")
+
+
 class CausalSelfAttention(nn.Module):
     def __init__(self, cfg: GPTConfig):
         super().__init__()
@@ -101,9 +114,11 @@ class CausalSelfAttention(nn.Module):
         self.attn_dropout, self.resid_dropout = nn.Dropout(cfg.dropout), nn.Dropout(cfg.dropout)
         self.n_head, self.n_embd, self.dropout = cfg.n_head, cfg.n_embd, cfg.dropout
 
-    def forward(self, x):
+    def forward(self, x, fused: bool = False, residual=None):
+        """``fused``: biases and ``residual`` in the projections' epilogues."""
         B, T, C = x.shape
-        q, k, v = self.c_attn(x).split(self.n_embd, dim=2)
+        qkv = ops.linear_act(x, self.c_attn.weight, self.c_attn.bias) if fused else self.c_attn(x)
+        q, k, v = qkv.split(self.n_embd, dim=2)
         D = C // self.n_head
         q, k, v = (t.view(B, T, self.n_head, D) for t in (q, k, v))
         if self.dropout > 0 and self.training:
@@ -111,7 +126,10 @@ class CausalSelfAttention(nn.Module):
                                                dropout_p=self.dropout, is_causal=True).transpose(1, 2)
         else:
             y = ops.flash_attn(q, k, v, causal=True)
-        return self.resid_dropout(self.c_proj(y.reshape(B, T, C)))
+        y = y.reshape(B, T, C)
+        if fused:
+            return self.resid_dropout(ops.linear_act(y, self.c_proj.weight, self.c_proj.bias, residual))
+        return self.resid_dropout(self.c_proj(y))
 
 
 class GELUMLP(nn.Module):
@@ -121,8 +139,34 @@ class GELUMLP(nn.Module):
         self.c_proj = nn.Linear(4 * cfg.n_embd, cfg.n_embd, bias=cfg.bias)
         self.dropout = nn.Dropout(cfg.dropout)
 
-    def forward(self, x):
+    def forward(self, x, fused: bool = False, residual=None):
+        if fused:
+            h = ops.linear_act(x, self.c_fc.weight, self.c_fc.bias, activation="gelu")
+            return self.dropout(ops.linear_act(h, self.c_proj.weight, self.c_proj.bias, residual))
         return self.dropout(self.c_proj(F.gelu(self.c_fc(x))))
+
+
+class Branch(nn.Module):
+    """How a block's output joins the residual stream: x + scale * gate * norm(h)."""
+
+    def __init__(self, cfg: GPTConfig):
+        super().__init__()
+        self.norm = LayerNorm(cfg.n_embd, cfg.bias) if cfg.post_norm else None
+        self.gate = nn.Parameter(torch.full((cfg.n_embd,), float(cfg.gate_init))) if cfg.residual_gate else None
+        self.scale = cfg.residual_scale
+        self.plain = not cfg.post_norm and not cfg.residual_gate and cfg.residual_scale == 1.0
+
+    def weights(self) -> dict:
+        n = self.norm
+        return dict(post_weight=None if n is None else n.weight, post_bias=None if n is None else n.bias, gate=self.gate,
+                    scale=self.scale)
+
+    def forward(self, x, h):
+        if self.plain:
+            return x + h
+        if self.norm is not None:
+            h = self.norm(h)
+        return x + self.scale * (h if self.gate is None else self.gate * h)
 
 
 class Block(nn.Module):
@@ -130,10 +174,30 @@ class Block(nn.Module):
         super().__init__()
         self.ln_1, self.attn = LayerNorm(cfg.n_embd, cfg.bias), CausalSelfAttention(cfg)
         self.ln_2, self.mlp = LayerNorm(cfg.n_embd, cfg.bias), GELUMLP(cfg)
+        self.join_1, self.join_2 = Branch(cfg), Branch(cfg)
+        self.fused_ops, self.dropout = cfg.fused_ops, cfg.dropout
 
     def forward(self, x):
-        x = x + self.attn(self.ln_1(x))
-        return x + self.mlp(self.ln_2(x))
+        if self.fused_ops and _fusable(x):
+            return self._fused(x)
+        x = self.join_1(x, self.attn(self.ln_1(x)))
+        return self.join_2(x, self.mlp(self.ln_2(x)))
+
+    def _fused(self, x):
+        """The same through the fused operators.  A plain branch adds the residual in its projection's
+        epilogue (one stream less than adding it with the norm), unless dropout comes between."""
+        drop = self.dropout > 0 and self.training
+        y, _ = ops.block_norm(x, kind="layer", pre_weight=self.ln_1.weight, pre_bias=self.ln_1.bias, eps=1e-5)
+        y, x = self._join(self.attn, self.join_1, y, x, self.ln_2, drop)
+        return self._join(self.mlp, self.join_2, y, x, None, drop)[1]
+
+    @staticmethod
+    def _join(block, branch, y, x, norm, drop):
+        w = {} if norm is None else dict(pre_weight=norm.weight, pre_bias=norm.bias)
+        if branch.plain and not drop:
+            x = block(y, fused=True, residual=x)
+            return ops.block_norm(x, kind="layer", eps=1e-5, **w)
+        return ops.block_norm(block(y, fused=True), x, kind="layer", eps=1e-5, **branch.weights(), **w)
 
 
 class MLPExperts(nn.Module):
@@ -254,11 +318,12 @@ class MoEBlock(nn.Module):
         super().__init__()
         self.ln_1, self.attn = LayerNorm(cfg.n_embd, cfg.bias), CausalSelfAttention(cfg)
         self.ln_2, self.mlp = LayerNorm(cfg.n_embd, cfg.bias), MOELayer(cfg)
+        self.join_1, self.join_2 = Branch(cfg), Branch(cfg)
 
     def forward(self, x):
-        x = x + self.attn(self.ln_1(x))
+        x = self.join_1(x, self.attn(self.ln_1(x)))
         m, loss = self.mlp(self.ln_2(x))
-        return x + m, loss
+        return self.join_2(x, m), loss
 
 
 class GPT(nn.Module):
