@@ -48,15 +48,13 @@ ST_DEVICE f32x4 unpack4(u32x2 p, bool f16) {
 ST_DEVICE float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 ST_DEVICE float rcp(float x) { return __builtin_amdgcn_rcpf(x); }
 ST_DEVICE float sigmoid(float x) { return rcp(1.f + exp2_(x * -1.4426950408889634f)); }
-// Phi(-|z|) and e = exp(-z^2 / 2)
-ST_DEVICE float normal_tail(float z, float& e) {
-  const float a = __builtin_fabsf(z);
+// p, t and e = exp(-z^2 / 2) with Phi(-|z|) = t p e
+ST_DEVICE float normal_poly(float z, float& e, float& t) {
   e = exp2_(z * (z * -0.72134752044448170f));
-  const float t = rcp(__builtin_fmaf(a, 0.23164190f, 1.f));
-  const float p = __builtin_fmaf(
+  t = rcp(__builtin_fmaf(__builtin_fabsf(z), 0.23164190f, 1.f));
+  return __builtin_fmaf(
       t, __builtin_fmaf(t, __builtin_fmaf(t, __builtin_fmaf(t, 0.5307027145f, -0.7265760135f), 0.7107068705f), -0.142248368f),
       0.127414796f);
-  return t * p * e;
 }
 constexpr float kTanhA = 1.5957691216057308f, kTanhB = 0.044715f;  // 2 sqrt(2 / pi): (1 + tanh(a)) / 2 = sigmoid(2 a)
 constexpr float kLog2e = 1.4426950408889634f;
@@ -64,10 +62,11 @@ constexpr float kLog2e = 1.4426950408889634f;
 ST_DEVICE float act_of(float z, int act) {
   float e;
   switch (act) {
-    case kRelu: return z > 0.f ? z : (z != z ? z : 0.f);
-    case kGelu: {  // z Phi(z) = max(z, 0) - |z| Phi(-|z|); the fabs of an infinite z times a zero tail is kept out
-      const float c = normal_tail(z, e), a = __builtin_fminf(__builtin_fabsf(z), 1e30f);
-      return (z > 0.f ? z : (z != z ? z : 0.f)) - a * c;
+    case kRelu: return z < 0.f ? 0.f : z;
+    case kGelu: {  // z Phi(z) = max(z, 0) - |z| Phi(-|z|); an infinite |z| times a zero tail is kept out
+      float t;
+      const float p = normal_poly(z, e, t);
+      return __builtin_fmaf(-__builtin_fminf(__builtin_fabsf(z), 1e30f), t * p * e, __builtin_fmaxf(z, 0.f));
     }
     case kGeluTanh: {
       const float s = z * __builtin_fmaf(z * z, -kTanhA * kTanhB * kLog2e, -kTanhA * kLog2e);
@@ -81,8 +80,8 @@ ST_DEVICE float act_slope(float z, int act) {
   switch (act) {
     case kRelu: return z > 0.f ? 1.f : (z != z ? z : 0.f);
     case kGelu: {
-      float e;
-      const float c = normal_tail(z, e);
+      float e, t;
+      const float p = normal_poly(z, e, t), c = t * p * e;
       return (z < 0.f ? c : 1.f - c) + z * e * 0.39894228040143268f;
     }
     case kGeluTanh: {

@@ -412,7 +412,7 @@ __global__ __launch_bounds__(NT, 1) void linear_wide_kernel(LinearArgs p, int gm
 }
 #pragma clang diagnostic pop
 
-// The parts of the cut tiles, in order, then their epilogue: four (i, j) blocks of a tile a workgroup.
+// The parts of the cut tiles, in order, then their epilogue: an (i, j) block of a tile a workgroup.
 __global__ __launch_bounds__(NT) void linear_wide_join_kernel(LinearArgs p, int gm, int nfull) {
   const int nbm = (p.M + BT - 1) / BT, nbn = (p.N + BT - 1) / BT, nv = nbm * nbn, tail = nv - nfull;
   const int id = xcd_remap(nfull + (int)blockIdx.x, nv), per = gm * nbn, grp = id / per, in = id % per;
@@ -420,15 +420,17 @@ __global__ __launch_bounds__(NT) void linear_wide_join_kernel(LinearArgs p, int 
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
   const int m0 = (grp * gm + in % gsz) * BT + (wid >> 1) * 128 + (lane & 15);
   const int n0 = (in / gsz) * BT + (wid & 1) * 128 + 4 * (lane >> 4);
+  const int ij = (int)blockIdx.y, m = m0 + 16 * (ij >> 3), n = n0 + 16 * (ij & 7);
+  const f32x4* w = reinterpret_cast<const f32x4*>(p.ws) + (int64_t)blockIdx.x * (BT * BT / 4) + ij * NT + threadIdx.x;
+  f32x4 part[8];  // all requested before the first sum
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const int ij = (int)blockIdx.y * 4 + k;
-    const f32x4* w = reinterpret_cast<const f32x4*>(p.ws) + (int64_t)blockIdx.x * (BT * BT / 4) + ij * NT + threadIdx.x;
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < p.splits; ++s) v += w[(int64_t)s * tail * (BT * BT / 4)];
-    const int m = m0 + 16 * (ij >> 3), n = n0 + 16 * (ij & 7);
-    if (m < p.M && n < p.N) epilogue4(p.epi, m, n, p.N - n, true, v);
-  }
+  for (int s = 0; s < 8; ++s)
+    if (s < p.splits) part[s] = w[(int64_t)s * tail * (BT * BT / 4)];
+  f32x4 v = part[0];
+#pragma unroll
+  for (int s = 1; s < 8; ++s)
+    if (s < p.splits) v += part[s];
+  if (m < p.M && n < p.N) epilogue4(p.epi, m, n, p.N - n, true, v);
 }
 
 int cu_count() {
@@ -444,8 +446,8 @@ int cu_count() {
 }
 
 // Tiles that are done whole, the parts that each of the others is cut into, and the time to expect.
-// Measured: a step of a tile takes some 1.6 us (24576 x 4096 x 14336), a round's epilogue 8; a part's
-// 256 KiB go out and come back through the cache at some 9 TB/s, and the second kernel costs 6 us.
+// Measured: a step of a tile takes some 1.6 us (24576 x 4096 x 14336), a round's epilogue 8, or 13 where
+// it writes fp32 parts; the second kernel reads those at some 4 TB/s and costs 6 us more.
 constexpr int kGroup = 4;
 struct WidePlan {
   int nfull, splits;
@@ -457,7 +459,7 @@ WidePlan linear_wide_plan(int M, int N, int K) {
   WidePlan best{nv, 1, rounds * (8.0 + 1.6 * KT)};
   for (int s = 2; tail && s <= 8 && KT / s >= 4; ++s) {
     const int parts = (tail * s + cus - 1) / cus;
-    const double us = rounds * 8.0 + 1.6 * ((rounds - 1) * KT + parts * ((KT + s - 1) / s)) + 6.0 + tail * s * 0.5243 / 9.0;
+    const double us = (rounds - 1) * (8.0 + 1.6 * KT) + parts * (13.0 + 1.6 * ((KT + s - 1) / s)) + 6.0 + tail * s * 0.2621 / 4.0;
     if (us < best.us) best = WidePlan{nv - tail, s, us};
   }
   return best;
@@ -476,7 +478,7 @@ int launch(const LinearArgs& p, hipStream_t st) {
   if (w.splits > 1) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
-    linear_wide_join_kernel<<<dim3((unsigned)(nv - w.nfull), 16), NT, 0, st>>>(q, kGroup, w.nfull);
+    linear_wide_join_kernel<<<dim3((unsigned)(nv - w.nfull), 64), NT, 0, st>>>(q, kGroup, w.nfull);
   }
   return (int)hipGetLastError();
 }
