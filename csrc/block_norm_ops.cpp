@@ -240,6 +240,7 @@ class BlockNorm : public torch::autograd::Function<BlockNorm> {
     ctx->saved_data["rtype"] = has(residual) ? (int64_t)residual->scalar_type() : (int64_t)-1;
     ctx->saved_data["has_y"] = has(w2);
     ctx->set_materialize_grads(false);
+    if (write_s && !(need & 31)) ctx->mark_non_differentiable({out[1]});  // nothing that s depends on wants a gradient
     torch::autograd::variable_list r;
     if (has(w2)) r.push_back(out[0]);
     if (write_s) r.push_back(out[1]);

@@ -176,6 +176,8 @@ class Block(nn.Module):
         self.ln_2, self.mlp = LayerNorm(cfg.n_embd, cfg.bias), GELUMLP(cfg)
         self.join_1, self.join_2 = Branch(cfg), Branch(cfg)
         self.fused_ops, self.dropout = cfg.fused_ops, cfg.dropout
+        if cfg.fused_ops:  # weights read without calling their modules: their buckets are waited for here
+            self._st_reads = (self.ln_1, self.attn, self.ln_2, self.mlp, self.join_1, self.join_2)
 
     def forward(self, x):
         if self.fused_ops and _fusable(x):

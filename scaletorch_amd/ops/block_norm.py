@@ -65,6 +65,8 @@ class _BlockNormFn(torch.autograd.Function):
         ctx.save_for_backward(*rows, stats, gate, w1, b1, w2, b2)
         ctx.meta = (layer, scale, eps, h.dtype, residual is not None, None if residual is None else residual.dtype)
         ctx.set_materialize_grads(False)
+        if write_s and not any(ctx.needs_input_grad[:5]):
+            ctx.mark_non_differentiable(s)
         return y, s
 
     @staticmethod

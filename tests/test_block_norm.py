@@ -301,6 +301,62 @@ def test_repeatable_streams_and_graphs():
         torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("need", [("h",), ("residual",), ("gate",), ("pre_weight",), ("post_bias", "pre_bias"), ("h", "post_weight")])
+def test_some_gradients_only(device, need):
+    c = _inputs(device, 40, 520, torch.bfloat16)
+    _, _, want = _run(c, "layer", 0.7)
+    t = {k: c[k].clone().requires_grad_(k in need) for k in NAMES}
+    y, s = ops.block_norm(t["h"], t["residual"], kind="layer", scale=0.7, eps=EPS, **{k: t[k] for k in NAMES[2:]})
+    outs = [(o, g) for o, g in ((y, c["dy"]), (s, c["ds"])) if o.requires_grad]
+    assert len(outs) == (1 if need == ("pre_weight",) else 2)  # s does not depend on the norm before the next block
+    for k, g in zip(need, torch.autograd.grad([o for o, _ in outs], [t[k] for k in need], [g for _, g in outs])):
+        assert torch.equal(g, want[k])
+    if device == "cuda":
+        y, s = ops.block_norm(t["h"], t["residual"], kind="layer", scale=0.7, eps=EPS, **{k: t[k] for k in NAMES[2:]})
+        with pytest.raises(RuntimeError, match="again"):
+            torch.autograd.grad(y, [t[need[0]]], c["dy"], create_graph=True)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_broadcast_residual_and_stream_used_twice(device):
+    c = _inputs(device, 12, 264, torch.float32)
+    r = c["residual"][:1].clone().requires_grad_(True)
+    h = c["h"].clone().requires_grad_(True)
+    y, s = ops.block_norm(h, r.expand(12, 264), kind="rms", pre_weight=c["pre_weight"], eps=EPS)
+    y2, s2 = ops.block_norm(y, s, kind="rms", pre_weight=c["pre_weight"], eps=EPS)
+    gh, gr = torch.autograd.grad((y2, s2), (h, r), (c["dy"], c["ds"]))
+    hd, rd = h.detach().double().requires_grad_(True), r.detach().double().requires_grad_(True)
+    w = c["pre_weight"].double()
+    a, b = block_norm_ref(hd, rd.expand(12, 264), False, None, None, None, 1.0, w, None, EPS)
+    a, b = block_norm_ref(a, b, False, None, None, None, 1.0, w, None, EPS)
+    dh, dr = torch.autograd.grad((a, b), (hd, rd), (c["dy"].double(), c["ds"].double()))
+    # a few hundred fp32 roundings of values of the gradients' size
+    assert ((gh.double() - dh).norm() / dh.norm()).item() <= 1e-5 and ((gr.double() - dr).norm() / dr.norm()).item() <= 1e-5
+
+
+@pytest.mark.gpu
+def test_rows_past_32_bits():
+    rows, width = 270000, 8192
+    if torch.cuda.mem_get_info()[0] < 40e9:
+        pytest.skip("needs 40 GB")
+    h = torch.zeros(rows, width, device="cuda", dtype=torch.bfloat16)
+    ends = torch.tensor([0, 1, rows // 2, rows - 2, rows - 1], device="cuda")
+    c = _inputs("cuda", 5, width, torch.bfloat16)
+    h[ends] = c["h"]
+    h.requires_grad_(True)
+    w = c["pre_weight"].requires_grad_(True)
+    y, _ = ops.block_norm(h, kind="rms", pre_weight=w, eps=EPS)
+    dy = torch.zeros_like(y)
+    dy[ends] = c["dy"]
+    dh, dw = torch.autograd.grad(y, (h, w), dy)
+    hs = c["h"].clone().requires_grad_(True)
+    ys, _ = ops.block_norm(hs, kind="rms", pre_weight=w, eps=EPS)
+    dhs, dws = torch.autograd.grad(ys, (hs, w), c["dy"])
+    assert torch.equal(y[ends], ys) and torch.equal(dh[ends], dhs) and not dh[2:rows // 2].any()
+    assert ((dw.double() - dws.double()).norm() / dws.double().norm()).item() <= 2.0 ** -8  # another order, rounded
+
+
 @pytest.mark.gpu
 def test_main_grad_takes_the_sums():
     c = _inputs("cuda", 300, 520, torch.bfloat16)

@@ -98,6 +98,64 @@ def test_training_steps_together(device, kind):
     assert all(not torch.equal(p, first[n]) for n, p in m.named_parameters() if n != "transformer.wpe.weight")
 
 
+def test_fused_weights_are_waited_for():
+    """The arena's bucket waits cover what the fused blocks read without calling its modules."""
+    from scaletorch_amd.parallel.data_parallel import DataParallel
+
+    idx = torch.randint(0, 97, (2, 16))
+    left = {}
+    for fused in (False, True):
+        dp = DataParallel(_model(fused, post_norm=True, residual_gate=True), expose_grads=True)
+        left[fused] = dp.uncovered_params(lambda: dp(idx, idx))
+    assert left[True] == left[False]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("kind", ["fp32", "fp8"])
+def test_in_data_parallel_arenas(device, kind):
+    """Parameters in arenas (views, fp32 main_grad): the gradients of the bare model and a step."""
+    from scaletorch_amd.parallel.data_parallel import DataParallel
+
+    idx = torch.randint(0, 97, (2, 32), device=device)
+    dt = torch.bfloat16 if device == "cuda" else torch.float32
+    bare, inner = (_model(True, post_norm=True, residual_gate=True).to(device, dt) for _ in range(2))
+    _, want = _grads(bare, idx)
+    dp = DataParallel(inner, bucket_size=1 << 16, expose_grads=True)
+    opt = inner.configure_optimizers(0.1, 1e-3, (0.9, 0.95), device, state_dtype=kind)
+    for _ in range(2):
+        dp.zero_grad()
+        dp(idx, idx)[1].backward()
+        got = {n: p.grad.double() for n, p in inner.named_parameters()}
+        # the arena keeps fp32 sums where the bare model rounds them to bf16 once
+        assert max(_off(got, want).values()) <= (2.0 ** -7 if device == "cuda" else 1e-5)
+    before = [p.detach().clone() for p in inner.parameters()]
+    opt.step()
+    assert all(torch.isfinite(p).all() for p in inner.parameters())
+    # the masters move: a step of 1e-3 is below half a bf16 step of a weight of one
+    now = [opt.state[p].get("master", p) for p in inner.parameters()]
+    assert all(not torch.equal(p, q.float()) for (n, _), p, q in zip(inner.named_parameters(), now, before) if "wpe" not in n)
+
+
+def test_mingpt_example_runs_fused_with_8_bit_states(tmp_path):
+    import subprocess
+    import sys
+
+    import yaml
+    root = __import__("os").path.dirname(__import__("os").path.dirname(__file__))
+    cfg = yaml.safe_load(open(f"{root}/examples/mingpt/gpt2_train_cfg.yaml"))
+    cfg["gpt_config"] |= dict(n_layer=2, n_head=2, n_embd=32, fused_ops=True, post_norm=True, residual_gate=True)
+    cfg["gpt_config"].pop("model_type", None)
+    cfg["data_config"] |= dict(block_size=32, truncate=0.2)
+    cfg["trainer_config"] |= dict(batch_size=4, max_epochs=1, data_loader_workers=0)
+    cfg["optimizer_config"]["state_dtype"] = "fp8"
+    (tmp_path / "c.yaml").write_text(yaml.safe_dump(cfg))
+    out = subprocess.run([sys.executable, f"{root}/examples/mingpt/main.py", "--cpu", "--max_iters", "3", "--config",
+                          str(tmp_path / "c.yaml"), "--snapshot_path", str(tmp_path / "s.pt")], capture_output=True,
+                         text=True, timeout=300, cwd=root)
+    assert out.returncode == 0, out.stderr[-2000:]
+    assert "final train loss" in out.stdout and "nan" not in out.stdout
+
+
 @pytest.mark.gpu
 def test_generation_one_token_at_a_time():
     """Few rows: the streaming product kernel, against the unfused model's choices at fp32 logits."""
