@@ -20,6 +20,15 @@ typedef __bf16 bfx4 __attribute__((ext_vector_type(4)));
 typedef _Float16 hx8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
+typedef __amdgpu_buffer_rsrc_t rsrc_t;
+constexpr uint32_t kOut = 0xffffffe0u;  // an offset behind every range: loads give zero, stores go nowhere
+ST_DEVICE uint32_t uni(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+ST_DEVICE rsrc_t rsrc_of(const void* base, uint32_t bytes) {  // of wave-uniform values
+  const uint64_t a = (uint64_t)base;
+  return __builtin_amdgcn_make_buffer_rsrc((void*)(((uint64_t)uni((uint32_t)(a >> 32)) << 32) | uni((uint32_t)a)),
+                                           (short)0, (int)uni(bytes), 0x00020000);
+}
+
 // 16-bit types travel as raw bits; F16 says which they are
 ST_DEVICE float half_up(uint32_t h, bool f16) {
   return f16 ? __half2float(__ushort_as_half((unsigned short)h)) : __uint_as_float(h << 16);

@@ -12,7 +12,7 @@
 using st::LinearArgs;
 
 extern "C" {
-int64_t st_linear_tile_ws(int M, int N, int K);
+int64_t st_linear_tile_ws(int M, int N, int K, int vec);
 int st_linear_tile(LinearArgs* p, int acol, int bcol, hipStream_t st);
 double st_linear_tile_us(int M, int N, int K);
 int st_linear_rows(const LinearArgs* p, hipStream_t st);
@@ -48,8 +48,6 @@ void product(const at::Tensor& A, bool acol, const at::Tensor& B, bool bcol, st:
              int64_t K, bool vec) {
   check_dims(M, N, K);
   LinearArgs p{};
-  p.a = A.data_ptr();
-  p.b = B.data_ptr();
   p.lda = ld_of(A);
   p.ldb = ld_of(B);
   p.M = (int)M;
@@ -60,7 +58,18 @@ void product(const at::Tensor& A, bool acol, const at::Tensor& B, bool bcol, st:
   p.epi = e;
   p.splits = 1;
   const int64_t ca = acol ? M : K, cb = bcol ? N : K;  // the contiguous dimension of each operand
-  p.vec = vec && ca % 8 == 0 && cb % 8 == 0 && N % 4 == 0 && p.lda % 8 == 0 && p.ldb % 8 == 0 && aligned(A) && aligned(B);
+  // an operand of fewer than 8 elements is read from a copy with room behind it
+  auto roomy = [](const at::Tensor& t, int64_t ld) {
+    if ((t.size(0) - 1) * ld + t.size(1) >= 8) return t;
+    auto b = at::zeros({16}, t.options());
+    b.as_strided(t.sizes(), {ld, 1}).copy_(t);
+    return b;
+  };
+  const at::Tensor ka = roomy(A, p.lda), kb = roomy(B, p.ldb);
+  p.a = ka.data_ptr();
+  p.b = kb.data_ptr();
+  const int64_t most = (int64_t)1 << 31;  // bytes that a descriptor of 128 rows spans
+  p.vec = vec && (p.lda * 128 + K) * 2 < most && (p.ldb * 128 + K) * 2 < most && ca % 8 == 0 && cb % 8 == 0 && N % 4 == 0 && p.lda % 8 == 0 && p.ldb % 8 == 0 && aligned(A) && aligned(B);
   int rc = -2;
   // few rows stream the weight; else whichever tiling is expected to be faster
   if (!acol && !bcol && M <= 64) rc = st_linear_rows(&p, stream());
@@ -68,7 +77,7 @@ void product(const at::Tensor& A, bool acol, const at::Tensor& B, bool bcol, st:
     const double wide = st_linear_wide_us(&p, acol, bcol);
     const bool use_wide = wide >= 0.0 && wide < st_linear_tile_us(p.M, p.N, p.K);
     at::Tensor ws;
-    if (const int64_t n = use_wide ? st_linear_wide_ws(&p) : st_linear_tile_ws(p.M, p.N, p.K)) {
+    if (const int64_t n = use_wide ? st_linear_wide_ws(&p) : st_linear_tile_ws(p.M, p.N, p.K, p.vec)) {
       ws = at::empty({n}, A.options().dtype(at::kFloat));
       p.ws = ws.data_ptr<float>();
     }

@@ -1,13 +1,14 @@
 // The product with its epilogue for every shape: BM x BN tiles, 2 x 2 waves, k in steps of 64.
 //
 // A step's operands go global -> registers (16-byte loads, or element by element where rows are not
-// aligned), issued a step ahead, then to one of two LDS images, from which the waves read their
-// MFMA fragments; one barrier a step.  kRow images are [rows][64 k], 16-byte chunk c of row r at
+// aligned), issued several steps ahead (a step of a small tile computes for 0.1 us, a load takes one),
+// then to one of two LDS images, from which the waves read their MFMA fragments; one barrier a step.  kRow images are [rows][64 k], 16-byte chunk c of row r at
 // c ^ ((r >> 1) & 7); kCol images [64 k][rows] in 256-byte (64-column tiles: 128-byte) rows, read
 // with the transposing LDS read, chunk c of row k at c ^ swz(k).  Chunks behind an operand's end
 // are zeros.  Few tiles: k is split over workgroups, whose fp32 sums a second kernel adds up in
 // order before the epilogue.
 #include <algorithm>
+#include <type_traits>
 
 #include "linear_act.h"
 
@@ -16,6 +17,7 @@ using namespace st;
 namespace {
 
 constexpr int BK = 64, NT = 256;
+typedef u32x4 __attribute__((aligned(2))) u32x4_any;  // 16 bytes at any element
 typedef __attribute__((address_space(3))) char lds_t;
 
 template <bool F16>
@@ -27,60 +29,79 @@ ST_DEVICE f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
 }
 
 // One operand of a tile: R rows (m or n), layout COL.
+//
+// Loads never branch, so that several steps of them stay in flight (behind a branch the compiler
+// waits for all of them).  VEC: through a buffer descriptor, lanes behind the operand's end at an
+// offset that reads as zero.  Else: 16 bytes from any element, moved back where they would run past
+// the operand's last one; the shift and the zeros follow when the chunk goes to LDS.
 template <int R, bool COL, bool VEC>
 struct Operand {
   static constexpr int kChunks = R * BK / 8 / NT;  // 16-byte chunks a thread moves
   static constexpr int kBytes = R * BK * 2;
-  const uint16_t* base;
-  int64_t ld;
-  int rows, K;
-  u32x4 reg[kChunks];
+  typedef u32x4 Regs[kChunks];  // one step's part of a thread
+  const uint16_t* base;         // of the tile's first row
+  int64_t ld, span;             // elements between rows (k), and from base to the operand's end
+  int rows, K;                  // rows from the tile's first on, all of k
 
   ST_DEVICE static int swz(int k) {  // kCol: spreads the 16 k rows of a transposed read over the banks
     return R == 128 ? ((k & 3) << 2) | ((k >> 2) & 3) : ((k & 1) << 2) | ((k >> 1) & 3);
   }
-  ST_DEVICE static int lds_at(int c) {  // byte of chunk c of the image
-    if constexpr (COL) {
-      constexpr int per = R / 8;
-      const int k = c / per, p = c % per;
-      return k * (R * 2) + 16 * (p ^ swz(k));
+  // row and k (within the step) of chunk i of this thread
+  ST_DEVICE static int row_of(int i) {
+    const int c = threadIdx.x + NT * i;
+    return COL ? (c % (R / 8)) * 8 : c >> 3;
+  }
+  ST_DEVICE static int k_of(int i) {
+    const int c = threadIdx.x + NT * i;
+    return COL ? c / (R / 8) : (c & 7) * 8;
+  }
+  ST_DEVICE static int lds_at(int i) {  // its byte in the image
+    const int r = row_of(i), k = k_of(i);
+    return COL ? k * (R * 2) + 16 * ((r >> 3) ^ swz(k)) : r * 128 + 16 * ((k >> 3) ^ ((r >> 1) & 7));
+  }
+  ST_DEVICE int64_t at(int i, int k0) const {
+    return COL ? (int64_t)(k0 + k_of(i)) * ld + row_of(i) : (int64_t)row_of(i) * ld + k0 + k_of(i);
+  }
+  ST_DEVICE int left(int i, int k0) const {  // elements of the chunk inside the operand; may be over 8 or below 0
+    return COL ? (k0 + k_of(i) < K ? rows - row_of(i) : 0) : (row_of(i) < rows ? K - k0 - k_of(i) : 0);
+  }
+  ST_DEVICE void load(int k0, Regs& reg) const {
+    if constexpr (VEC) {
+      const int most = min(R, rows);
+      const rsrc_t rs = COL ? rsrc_of(base + (int64_t)k0 * ld, (uint32_t)(((int64_t)(min(BK, K - k0) - 1) * ld + most) * 2))
+                            : rsrc_of(base, (uint32_t)(((int64_t)(most - 1) * ld + K) * 2));
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) {
+        const uint32_t off = (uint32_t)(((COL ? (int64_t)k_of(i) * ld + row_of(i) : (int64_t)row_of(i) * ld + k_of(i)) * 2));
+        reg[i] = __builtin_amdgcn_raw_buffer_load_b128(rs, left(i, k0) > 0 ? off : kOut, COL ? 0 : k0 * 2, 0);
+      }
     } else {
-      const int r = c >> 3, p = c & 7;
-      return r * 128 + 16 * (p ^ ((r >> 1) & 7));
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) {
+        const int64_t a = left(i, k0) > 0 ? at(i, k0) : 0;
+        reg[i] = *reinterpret_cast<const u32x4_any*>(base + min(a, span - 8));  // the operand has 8 elements or more
+      }
     }
   }
-  ST_DEVICE void load(int k0, int kend) {
+  ST_DEVICE void store(lds_t* img, int k0, const Regs& reg) const {
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
-      const int c = threadIdx.x + NT * i;
-      int r, k;
-      if constexpr (COL) {
-        k = k0 + c / (R / 8);
-        r = (c % (R / 8)) * 8;
-      } else {
-        r = c >> 3;
-        k = k0 + (c & 7) * 8;
-      }
-      const int64_t at = COL ? (int64_t)k * ld + r : (int64_t)r * ld + k;
-      u32x4 v = {0u, 0u, 0u, 0u};
-      if constexpr (VEC) {
-        if (r < rows && k < kend) v = *reinterpret_cast<const u32x4*>(base + at);
-      } else {
-        uint32_t e[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const bool in = COL ? (k < kend && r + j < rows) : (r < rows && k + j < kend);
-          e[j] = in ? base[at + j] : 0u;
+      u32x4 v = reg[i];
+      if constexpr (!VEC) {
+        const int n = left(i, k0), d = n > 0 ? (int)max((int64_t)0, at(i, k0) - (span - 8)) : 0;
+        uint64_t lo = (uint64_t)v[1] << 32 | v[0], hi = (uint64_t)v[3] << 32 | v[2];
+        if (d > 0) {  // the chunk was read d elements early
+          lo = d >= 4 ? hi >> (16 * (d & 3)) : lo >> (16 * d) | hi << (64 - 16 * d);
+          hi = d >= 4 ? 0 : hi >> (16 * d);
         }
-        v = u32x4{e[0] | (e[1] << 16), e[2] | (e[3] << 16), e[4] | (e[5] << 16), e[6] | (e[7] << 16)};
+        if (n < 8) {
+          hi = n > 4 ? hi & ~(~0ull << (16 * (n - 4))) : 0;
+          lo = n >= 4 ? lo : n > 0 ? lo & ~(~0ull << (16 * n)) : 0;
+        }
+        v = u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
       }
-      reg[i] = v;
+      *reinterpret_cast<u32x4 __attribute__((address_space(3)))*>(img + lds_at(i)) = v;
     }
-  }
-  ST_DEVICE void store(lds_t* img) const {
-#pragma unroll
-    for (int i = 0; i < kChunks; ++i)
-      *reinterpret_cast<u32x4 __attribute__((address_space(3)))*>(img + lds_at(threadIdx.x + NT * i)) = reg[i];
   }
   // fragment of rows r0 .. r0 + 15, k 32 ks .. + 31: lane (g = lane / 16) holds k 8 g .. 8 g + 7 of row lane % 16
   ST_DEVICE static u32x4 frag(const lds_t* img, int r0, int ks) {
@@ -104,7 +125,8 @@ struct Operand {
   }
 };
 
-template <int BM, int BN, bool ACOL, bool BCOL, bool VEC, bool F16>
+// AHEAD: steps whose loads are in flight in registers (even: the LDS image of a step is then known)
+template <int BM, int BN, int AHEAD, bool ACOL, bool BCOL, bool VEC, bool F16>
 __global__ __launch_bounds__(NT) void linear_tile_kernel(LinearArgs p) {
   constexpr int WM = BM / 2, WN = BN / 2, FM = WM / 16, FN = WN / 16;
   typedef Operand<BM, ACOL, VEC> OpA;
@@ -129,44 +151,63 @@ __global__ __launch_bounds__(NT) void linear_tile_kernel(LinearArgs p) {
   B.ld = p.ldb;
   A.rows = p.M - m0;
   B.rows = p.N - n0;
+  A.K = B.K = p.K;
+  A.span = ACOL ? (int64_t)(p.K - 1) * p.lda + A.rows : (int64_t)(A.rows - 1) * p.lda + p.K;
+  B.span = BCOL ? (int64_t)(p.K - 1) * p.ldb + B.rows : (int64_t)(B.rows - 1) * p.ldb + p.K;
   f32x4 acc[FM][FN];
 #pragma unroll
   for (int i = 0; i < FM; ++i)
 #pragma unroll
     for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   constexpr int kStage = OpA::kBytes + OpB::kBytes;
-  if (s0 < s1) {
-    A.load(s0 * BK, p.K);
-    B.load(s0 * BK, p.K);
-    A.store(smem);
-    B.store(smem + OpA::kBytes);
-  }
-  __syncthreads();
-  for (int s = s0; s < s1; ++s) {
-    const lds_t* cur = smem + ((s - s0) & 1) * kStage;
-    lds_t* nxt = smem + ((s - s0 + 1) & 1) * kStage;
-    if (s + 1 < s1) {
-      A.load((s + 1) * BK, p.K);
-      B.load((s + 1) * BK, p.K);
+  typename OpA::Regs ra[AHEAD];
+  typename OpB::Regs rb[AHEAD];
+  const int n = s1 - s0;
+#pragma unroll
+  for (int j = 0; j < AHEAD; ++j)
+    if (j < n) {
+      A.load((s0 + j) * BK, ra[j]);
+      B.load((s0 + j) * BK, rb[j]);
     }
+  // step i's operands from registers i % AHEAD to image i % 2, and the registers on to step i + AHEAD
+  auto stage = [&](auto j_c, int i) {
+    constexpr int j = decltype(j_c)::value;
+    A.store(smem + (j & 1) * kStage, (s0 + i) * BK, ra[j]);
+    B.store(smem + (j & 1) * kStage + OpA::kBytes, (s0 + i) * BK, rb[j]);
+    if (i + AHEAD < n) {
+      A.load((s0 + i + AHEAD) * BK, ra[j]);
+      B.load((s0 + i + AHEAD) * BK, rb[j]);
+    }
+  };
+  if (n > 0) stage(std::integral_constant<int, 0>(), 0);
+  __syncthreads();
+  auto step = [&](auto j_c, int i) {
+    constexpr int j = decltype(j_c)::value;
+    const lds_t* cur = smem + (j & 1) * kStage;
+    // the other image was read a step ago, before the last barrier
+    if (i + 1 < n) stage(std::integral_constant<int, (j + 1) % AHEAD>(), i + 1);
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       u32x4 fa[FM], fb[FN];
 #pragma unroll
-      for (int i = 0; i < FM; ++i) fa[i] = OpA::frag(cur, wm * WM + 16 * i, ks);
+      for (int q = 0; q < FM; ++q) fa[q] = OpA::frag(cur, wm * WM + 16 * q, ks);
 #pragma unroll
-      for (int j = 0; j < FN; ++j) fb[j] = OpB::frag(cur + OpA::kBytes, wn * WN + 16 * j, ks);
+      for (int q = 0; q < FN; ++q) fb[q] = OpB::frag(cur + OpA::kBytes, wn * WN + 16 * q, ks);
       // operands swapped: a lane holds 4 consecutive columns of one row
 #pragma unroll
-      for (int i = 0; i < FM; ++i)
+      for (int q = 0; q < FM; ++q)
 #pragma unroll
-        for (int j = 0; j < FN; ++j) acc[i][j] = mfma<F16>(fb[j], fa[i], acc[i][j]);
-    }
-    if (s + 1 < s1) {
-      A.store(nxt);
-      B.store(nxt + OpA::kBytes);
+        for (int r = 0; r < FN; ++r) acc[q][r] = mfma<F16>(fb[r], fa[q], acc[q][r]);
     }
     __syncthreads();
+  };
+  for (int i = 0; i < n; i += AHEAD) {
+    step(std::integral_constant<int, 0>(), i);
+    if (i + 1 < n) step(std::integral_constant<int, 1>(), i + 1);
+    if constexpr (AHEAD > 2) {
+      if (i + 2 < n) step(std::integral_constant<int, 2>(), i + 2);
+      if (i + 3 < n) step(std::integral_constant<int, 3>(), i + 3);
+    }
   }
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
@@ -214,17 +255,17 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs p) {
   epilogue4(p.epi, m, n, p.N - n, p.vec != 0, v);
 }
 
-template <int B, bool ACOL, bool BCOL>
+template <int B, bool ACOL, bool BCOL, int AHEAD = B == 64 ? 4 : 2>
 int launch(const LinearArgs& p, hipStream_t st) {
   const int64_t tiles = (int64_t)((p.M + B - 1) / B) * ((p.N + B - 1) / B);
   if (tiles >= (1LL << 31)) return -2;
   const dim3 grid((unsigned)tiles, (unsigned)p.splits);
   if (p.vec) {
-    if (p.epi.f16) linear_tile_kernel<B, B, ACOL, BCOL, true, true><<<grid, NT, 0, st>>>(p);
-    else linear_tile_kernel<B, B, ACOL, BCOL, true, false><<<grid, NT, 0, st>>>(p);
-  } else {
-    if (p.epi.f16) linear_tile_kernel<B, B, ACOL, BCOL, false, true><<<grid, NT, 0, st>>>(p);
-    else linear_tile_kernel<B, B, ACOL, BCOL, false, false><<<grid, NT, 0, st>>>(p);
+    if (p.epi.f16) linear_tile_kernel<B, B, AHEAD, ACOL, BCOL, true, true><<<grid, NT, 0, st>>>(p);
+    else linear_tile_kernel<B, B, AHEAD, ACOL, BCOL, true, false><<<grid, NT, 0, st>>>(p);
+  } else if constexpr (B == 64) {
+    if (p.epi.f16) linear_tile_kernel<B, B, AHEAD, ACOL, BCOL, false, true><<<grid, NT, 0, st>>>(p);
+    else linear_tile_kernel<B, B, AHEAD, ACOL, BCOL, false, false><<<grid, NT, 0, st>>>(p);
   }
   if (p.splits > 1) {
     const hipError_t e = hipGetLastError();
@@ -240,10 +281,10 @@ int launch(const LinearArgs& p, hipStream_t st) {
 struct Plan {
   int tile, splits;
 };
-Plan plan(int M, int N, int K) {
+Plan plan(int M, int N, int K, int vec) {
   auto tiles = [&](int b) { return (int64_t)((M + b - 1) / b) * ((N + b - 1) / b); };
   const int steps = (K + BK - 1) / BK;
-  Plan r{tiles(128) >= 256 ? 128 : 64, 1};
+  Plan r{vec && tiles(128) >= 256 ? 128 : 64, 1};  // shifted loads leave 128 x 128 no registers for two a SIMD
   const int64_t t = tiles(r.tile);
   if (t < 512 && steps >= 8) r.splits = (int)std::min<int64_t>({(512 + t - 1) / t, steps / 4, 32});
   return r;
@@ -258,8 +299,8 @@ extern "C" {
 double st_linear_tile_us(int M, int N, int K) { return 4.0 + 2.0 * M * N * K / 5e8; }
 
 // fp32 workspace elements of a product.
-int64_t st_linear_tile_ws(int M, int N, int K) {
-  const Plan r = plan(M, N, K);
+int64_t st_linear_tile_ws(int M, int N, int K, int vec) {
+  const Plan r = plan(M, N, K, vec);
   return r.splits > 1 ? (int64_t)r.splits * M * N : 0;
 }
 
@@ -267,7 +308,7 @@ int64_t st_linear_tile_ws(int M, int N, int K) {
 // floats.  -2: outside the kernel's.
 int st_linear_tile(LinearArgs* p, int acol, int bcol, hipStream_t st) {
   if (p->M <= 0 || p->N <= 0 || p->K <= 0 || (acol && !bcol)) return -2;
-  const Plan r = plan(p->M, p->N, p->K);
+  const Plan r = plan(p->M, p->N, p->K, p->vec);
   p->splits = r.splits;
   if (r.splits > 1 && !p->ws) return -2;
   if (r.tile == 128) {

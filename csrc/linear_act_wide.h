@@ -43,7 +43,6 @@ constexpr int STAGE = 2 * IMG;
 ST_DEVICE int rsw(int r) { return (r >> 1) & 7; }
 ST_DEVICE int swz(int k) { return ((k & 3) << 2) | ((k >> 2) & 3); }
 ST_DEVICE void fence() { __builtin_amdgcn_sched_barrier(0); }
-ST_DEVICE uint32_t uni(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
 
 ST_DEVICE srd_t make_srd(const void* base, uint32_t bytes) {
   const uint64_t a = (uint64_t)base;
@@ -61,14 +60,6 @@ ST_DEVICE void static_for(F&& f) {
     f(std::integral_constant<int, B>());
     static_for<B + 1, E>(f);
   }
-}
-
-typedef __amdgpu_buffer_rsrc_t rsrc_t;
-constexpr uint32_t kOut = 0xffffffe0u;  // an offset that is out of every range
-ST_DEVICE rsrc_t rsrc_of(const void* base, uint32_t bytes) {
-  const uint64_t a = (uint64_t)base;
-  return __builtin_amdgcn_make_buffer_rsrc((void*)(((uint64_t)uni((uint32_t)(a >> 32)) << 32) | uni((uint32_t)a)),
-                                           (short)0, (int)uni(bytes), 0x00020000);
 }
 
 #pragma clang diagnostic push

@@ -74,6 +74,16 @@ def adamw_unpack8(exp_avg: torch.Tensor, root: torch.Tensor, scales: torch.Tenso
     return m, r * r
 
 
+def _some(ts):
+    """A list for the kernel's side, which takes tensors only: empty for none, an empty tensor in a None's place."""
+    if ts is None:
+        return []
+    if all(t is not None for t in ts):
+        return ts
+    none = next((t for t in ts if t is not None), None)
+    return [] if none is None else [none.new_empty(0) if t is None else t for t in ts]
+
+
 def _check(params, grads, exp_avg, exp_avg_sq, masters, scales, clip_coef, wd, scale_grads) -> None:
     """The checks of csrc/adamw_multi_ops.cpp, for CPU tensors."""
     n = len(params)
@@ -174,7 +184,6 @@ def adamw_multi_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], 
     step runs on the current stream; it takes its number from the host, so it can't be captured
     into a graph.
     """
-    params, grads = list(params), list(grads)
     n = len(params)
     if step < 1:
         raise ValueError(f"adamw_multi: step counts from 1, got {step}")
@@ -182,25 +191,19 @@ def adamw_multi_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], 
     if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
         raise ValueError(f"adamw_multi: betas must be in [0, 1), got {betas}")
     wd = [float(weight_decay)] * n if isinstance(weight_decay, (int, float)) else [float(w) for w in weight_decay]
-    masters = [None] * n if masters is None else list(masters)
-    scales = [None] * n if scales is None else list(scales)
     if not n:
         return
     if _lib.use_native(params[0]):
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("adamw_multi: the step number is the host's, so a captured step would repeat it; "
                                "run the step outside the graph")
-        if any(t is None for t in masters):
-            none = params[0].new_empty(0, dtype=torch.float32)
-            masters = [] if all(t is None for t in masters) else [none if t is None else t for t in masters]
-        if any(t is None for t in scales):
-            none = params[0].new_empty(0, dtype=torch.float32)
-            scales = [] if all(t is None for t in scales) else [none if t is None else t for t in scales]
-        _lib.ops().adamw_multi_(params, grads, list(exp_avg), list(exp_avg_sq), masters, scales, clip_coef, wd, lr,
-                                b1, b2, eps, step, scale_grads)
+        _lib.ops().adamw_multi_.default(params, grads, exp_avg, exp_avg_sq, _some(masters), _some(scales), clip_coef,
+                                        wd, lr, b1, b2, eps, step, scale_grads)
         # the kernel writes behind autograd's back: a graph that saved a parameter has to notice
         torch.autograd.graph.increment_version(params)
         return
+    masters = [None] * n if masters is None else masters
+    scales = [None] * n if scales is None else scales
     _check(params, grads, exp_avg, exp_avg_sq, masters, scales, clip_coef, wd, scale_grads and clip_coef is not None)
     _adamw_multi_ref(params, grads, exp_avg, exp_avg_sq, masters, scales, clip_coef, wd, lr, b1, b2, eps, step,
                      scale_grads)
