@@ -192,7 +192,7 @@ __global__ __launch_bounds__(1024) void block_norm_finish_kernel(FinishArgs f) {
     for (int b = 0; b < kParts; ++b)
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        if (k < f.arrays) s[k] += f.sums[((int64_t)b * f.arrays + k) * f.width + col];
+        s[k] += f.sums[((int64_t)b * f.arrays + (k < f.arrays ? k : 0)) * f.width + col];  // no branch: all in flight
     const float A = s[1], dyb = s[f.gen ? 2 : 1], B = s[3];
     if (f.dw2) put<T>(f.dw2, f.tw2, col, s[0]);
     if (f.db2) put<T>(f.db2, f.tb2, col, dyb);

@@ -106,6 +106,28 @@ ST_DEVICE float act_slope(float z, int act) {
   }
 }
 
+ST_DEVICE void act4(f32x4& v, int act) {  // one choice for four values
+  switch (act) {
+    case kRelu:
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = act_of(v[i], kRelu);
+      break;
+    case kGelu:
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = act_of(v[i], kGelu);
+      break;
+    case kGeluTanh:
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = act_of(v[i], kGeluTanh);
+      break;
+    case kSilu:
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = act_of(v[i], kSilu);
+      break;
+    default: break;
+  }
+}
+
 // The epilogue of four consecutive columns n .. n + 3 of row m (count of them inside the matrix;
 // vec: all four, with aligned rows).
 ST_DEVICE void epilogue4(const LinearEpi& e, int64_t m, int n, int count, bool vec, f32x4 v) {
@@ -113,10 +135,7 @@ ST_DEVICE void epilogue4(const LinearEpi& e, int64_t m, int n, int count, bool v
   if (vec && count >= 4) {
     if (e.bias) v += unpack4(*reinterpret_cast<const u32x2*>((const uint16_t*)e.bias + n), e.f16);
     if (e.z) *reinterpret_cast<u32x2*>((uint16_t*)e.z + at) = pack4(v, e.f16);
-    if (e.act) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = act_of(v[i], e.act);
-    }
+    act4(v, e.act);
     if (e.res)
       v += e.out_f32 ? *reinterpret_cast<const f32x4*>((const float*)e.res + at)
                      : unpack4(*reinterpret_cast<const u32x2*>((const uint16_t*)e.res + at), e.f16);

@@ -277,7 +277,9 @@ int launch(const LinearArgs& p, hipStream_t st) {
   return (int)hipGetLastError();
 }
 
-// Tile edge and splits of a product.
+// Tile edge and splits of a product.  Measured, us (forward, bias and GELU in brackets): splitting 256 tiles
+// costs where k is short -- 2048 x 512 x 2048 15 (23) whole, 26 (28) in two; 1024^3 10 (12) and 15 (17) --
+// and pays where it is long: 1000 x 4096 x 1000 30 (32) and 25 (25); 128 x 4096 x 4096, 128 tiles in four, 17.
 struct Plan {
   int tile, splits;
 };
@@ -286,7 +288,7 @@ Plan plan(int M, int N, int K, int vec) {
   const int steps = (K + BK - 1) / BK;
   Plan r{vec && tiles(128) >= 256 ? 128 : 64, 1};  // shifted loads leave 128 x 128 no registers for two a SIMD
   const int64_t t = tiles(r.tile);
-  if (t < 512 && steps >= 8) r.splits = (int)std::min<int64_t>({(512 + t - 1) / t, steps / 4, 32});
+  if (steps >= 8 && (t < 256 || (t < 512 && steps >= 48))) r.splits = (int)std::min<int64_t>({(512 + t - 1) / t, steps / 4, 32});
   return r;
 }
 
