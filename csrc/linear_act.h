@@ -86,6 +86,8 @@ ST_DEVICE float act_of(float z, int act) {
   }
 }
 ST_DEVICE float act_slope(float z, int act) {
+  // an fp16 z can have become infinite in storage: its slope is the limit, 0 or 1, not inf * 0
+  z = __builtin_fabsf(z) > 1e30f ? __builtin_copysignf(1e30f, z) : z;
   switch (act) {
     case kRelu: return z > 0.f ? 1.f : (z != z ? z : 0.f);
     case kGelu: {

@@ -40,7 +40,8 @@ at::Tensor rows_of(const at::Tensor& t) {
 int64_t ld_of(const at::Tensor& m) { return m.size(0) <= 1 ? m.size(1) : m.stride(0); }
 
 void check_dims(int64_t m, int64_t n, int64_t k) {
-  TORCH_CHECK_VALUE(m <= INT32_MAX && n <= INT32_MAX && k <= INT32_MAX, "linear_act: dimensions below 2^31");
+  const int64_t most = INT32_MAX - 511;  // rounding up to tiles stays in 32 bits
+  TORCH_CHECK_VALUE(m <= most && n <= most && k <= most, "linear_act: dimensions of at most ", most);
 }
 
 // C [M, N] = A B^T with the epilogue e (its out set); A, B 2-D, acol / bcol: stored [k, rows].
@@ -69,7 +70,8 @@ void product(const at::Tensor& A, bool acol, const at::Tensor& B, bool bcol, st:
   p.a = ka.data_ptr();
   p.b = kb.data_ptr();
   const int64_t most = (int64_t)1 << 31;  // bytes that a descriptor of 128 rows spans
-  p.vec = vec && (p.lda * 128 + K) * 2 < most && (p.ldb * 128 + K) * 2 < most && ca % 8 == 0 && cb % 8 == 0 && N % 4 == 0 && p.lda % 8 == 0 && p.ldb % 8 == 0 && aligned(A) && aligned(B);
+  p.vec = vec && (p.lda * 128 + K) * 2 < most && (p.ldb * 128 + K) * 2 < most && ca % 8 == 0 && cb % 8 == 0 &&
+          N % 4 == 0 && p.lda % 8 == 0 && p.ldb % 8 == 0 && aligned(A) && aligned(B);
   int rc = -2;
   // few rows stream the weight; else whichever tiling is expected to be faster
   if (!acol && !bcol && M <= 64) rc = st_linear_rows(&p, stream());

@@ -144,6 +144,30 @@ def test_activation_range(device, act):
     assert got[0, 0] == float("inf") and got[0, 1].isnan() and got[0, 3] > 9e29 and got[0, 4] == 0 and (got[0, 5:] > 1.5).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["relu", "gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("rows", [2, 300])
+def test_sums_past_fp16_range(act, rows):
+    """z = 262144 and -262144: finite in y (fp32), beyond what fp16 keeps for the backward.  Every value
+    here is exact: slopes of 1 and 0, and sums of powers of two."""
+    x = torch.full((rows, 1024), 256.0, device="cuda").half().requires_grad_(True)
+    w = torch.ones(8, 1024, device="cuda").half()
+    w[1::2] = -1
+    w.requires_grad_(True)
+    y = ops.linear_act(x, w, residual=torch.zeros(rows, 8, device="cuda"), activation=act)
+    assert (y[:, ::2] == 262144.0).all() and (y[:, 1::2] == 0).all()
+    dx, dw = torch.autograd.grad(y, [x, w], torch.full_like(y, 2.0 ** -10))
+    assert (dx == 2.0 ** -8).all()
+    assert (dw[::2] == rows / 4).all() and (dw[1::2] == 0).all()
+
+
+@pytest.mark.gpu
+def test_dimensions_past_the_limit_are_refused():
+    x = torch.empty(2 ** 31 - 1, 1, device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="at most"):
+        ops.linear_act(x, torch.ones(1, 1, device="cuda", dtype=torch.bfloat16))
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_layouts(device):
     """More dimensions, padded rows, shifted starts, columns of a wider tensor, a transposed weight, no rows."""
