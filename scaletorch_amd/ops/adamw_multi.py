@@ -200,7 +200,7 @@ def adamw_multi_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], 
         _lib.ops().adamw_multi_.default(params, grads, exp_avg, exp_avg_sq, _some(masters), _some(scales), clip_coef,
                                         wd, lr, b1, b2, eps, step, scale_grads)
         # the kernel writes behind autograd's back: a graph that saved a parameter has to notice
-        torch.autograd.graph.increment_version(params)
+        torch.autograd.graph.increment_version([*params, *grads] if scale_grads else params)
         return
     masters = [None] * n if masters is None else masters
     scales = [None] * n if scales is None else scales
