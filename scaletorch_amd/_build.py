@@ -30,15 +30,15 @@ LIB = PKG / "_st_kernels.so"
 ARCH = os.environ.get("PYTORCH_ROCM_ARCH", "gfx950").split(";")[0] or "gfx950"
 ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 
+# No packed fp32 arithmetic (v_pk_add / mul / fma_f32, which -O3 forms from ordinary float
+# code): some of its forms have given wrong results on MI355X.  The host pass warns that it
+# does not know the feature; it has no effect there.
+HIP_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # Per-file flags.  flash_attn: scores never hold NaN by construction (masked
 # entries are -inf, never inf - inf), so -fno-honor-nans drops the v_max
 # canonicalisation hipcc inserts before every fmaxf on an MFMA result;
 # -amdgpu-mfma-vgpr-form keeps compiler-emitted MFMAs in VGPRs (their results
 # feed VALU) while the asm accumulate chains own the AGPRs (see mfma_acc).
-# No packed fp32 arithmetic (v_pk_add / mul / fma_f32, which -O3 forms from ordinary float
-# code): some of its forms have given wrong results on MI355X.  The host pass warns that it
-# does not know the feature; it has no effect there.
-HIP_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 FILE_FLAGS = {"flash_attn.hip": ["-fno-honor-nans", "-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 

@@ -53,7 +53,7 @@ class GPTConfig:
     use_einsum_aggregation: bool = True
     expert_capacity_roundup: bool = True
     # blocks through the fused operators (ops.linear_act, ops.block_norm): bias, GELU and residual in the
-    # products' epilogues, LayerNorm as one kernel
+    # products' epilogues, LayerNorm as one kernel (expert blocks stay as they are)
     fused_ops: bool = False
     # residual branches: a norm after the block too, a learned gate a channel (from `gate_init`), a scale
     post_norm: bool = False
