@@ -12,7 +12,7 @@
 using st::LinearArgs;
 
 extern "C" {
-int64_t st_linear_tile_ws(int M, int N, int K, int vec);
+int64_t st_linear_tile_ws(int M, int N, int K, int vec, int acol, int bcol);
 int st_linear_tile(LinearArgs* p, int acol, int bcol, hipStream_t st);
 double st_linear_tile_us(int M, int N, int K);
 int st_linear_rows(const LinearArgs* p, hipStream_t st);
@@ -79,7 +79,7 @@ void product(const at::Tensor& A, bool acol, const at::Tensor& B, bool bcol, st:
     const double wide = st_linear_wide_us(&p, acol, bcol);
     const bool use_wide = wide >= 0.0 && wide < st_linear_tile_us(p.M, p.N, p.K);
     at::Tensor ws;
-    if (const int64_t n = use_wide ? st_linear_wide_ws(&p) : st_linear_tile_ws(p.M, p.N, p.K, p.vec)) {
+    if (const int64_t n = use_wide ? st_linear_wide_ws(&p) : st_linear_tile_ws(p.M, p.N, p.K, p.vec, acol, bcol)) {
       ws = at::empty({n}, A.options().dtype(at::kFloat));
       p.ws = ws.data_ptr<float>();
     }

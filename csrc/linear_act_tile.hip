@@ -3,15 +3,16 @@
 // A step's operands go global -> registers (16-byte loads, or element by element where rows are not
 // aligned), issued several steps ahead (a step of a small tile computes for 0.1 us, a load takes one),
 // then to one of two LDS images, from which the waves read their MFMA fragments; one barrier a step.
-// kRow images are [rows][64 k], 16-byte chunk c of row r at c ^ ((r >> 1) & 7); kCol images [64 k][rows] in 256-byte (64-column tiles: 128-byte) rows, read
-// with the transposing LDS read, chunk c of row k at c ^ swz(k).  Chunks behind an operand's end
-// are zeros.  Few tiles: k is split over workgroups, whose fp32 sums a second kernel adds up in
+// kRow images are [rows][64 k], 16-byte chunk c of row r at c ^ ((r >> 1) & 7); kCol images [64 k][rows]
+// in 256-byte (64-column tiles: 128-byte) rows, read with the transposing LDS read, chunk c of row k at
+// c ^ swz(k).  Chunks behind an operand's end are zeros.  Few tiles: k is split over workgroups, whose fp32 sums a second kernel adds up in
 // order before the epilogue.
 //
-// Bound by LDS (64 x 64 a wave moves 1.5 bytes for one that the matrix units could wait for) and, in
-// 64 x 64 tiles, by L2.  Measured, bf16: 2048^3 33 us (525 TF/s; the library's product 26), 4096 x 1024 x
-// 4096 53 us (650 TF/s; 34), 777 x 1000 x 2504 with the epilogue 21 us (the library's product alone 22),
-// 777 x 1001 x 2503 26 us, 24576 x 4096 x 14336 3.39 ms (850 TF/s).
+// Bound by a step's chain (LDS writes, barrier, fragments: 0.27 us for a 64 x 64 tile alone on its CU, of it 0.06
+// of matrix instructions) where there are few tiles, by the L1s where several share a CU.  Measured, bf16: 2048^3 33 us (520 TF/s; the library's product 26), its
+// gradients 31 (28-30), 1024^3 9 us (the library's product 21-25), 777 x 1000 x 2504 with the epilogue 20 us
+// (22 alone), 777 x 1001 x 2503 25 us, 24576 x 4096 x 14336 3.1 ms (930 TF/s).  With loads that some paths skip
+// every fourth step of the loop waited for all of them: dx of 2048^3 took 33 us and not 29.
 #include <algorithm>
 #include <type_traits>
 
@@ -73,7 +74,7 @@ struct Operand {
   ST_DEVICE void load(int k0, Regs& reg) const {
     if constexpr (VEC) {
       const int most = min(R, rows);
-      const rsrc_t rs = COL ? rsrc_of(base + (int64_t)k0 * ld, (uint32_t)(((int64_t)(min(BK, K - k0) - 1) * ld + most) * 2))
+      const rsrc_t rs = COL ? rsrc_of(base + (int64_t)k0 * ld, k0 < K ? (uint32_t)(((int64_t)(min(BK, K - k0) - 1) * ld + most) * 2) : 0u)
                             : rsrc_of(base, (uint32_t)(((int64_t)(most - 1) * ld + K) * 2));
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
@@ -168,29 +169,33 @@ __global__ __launch_bounds__(NT) void linear_tile_kernel(LinearArgs p) {
   typename OpA::Regs ra[AHEAD];
   typename OpB::Regs rb[AHEAD];
   const int n = s1 - s0;
+  // Steps behind the last are loaded too (zeros behind k's end, or the next part's values, which nothing
+  // reads): where loads are skipped on some path the compiler waits as if none had followed.
 #pragma unroll
-  for (int j = 0; j < AHEAD; ++j)
-    if (j < n) {
-      A.load((s0 + j) * BK, ra[j]);
-      B.load((s0 + j) * BK, rb[j]);
-    }
+  for (int j = 0; j < AHEAD; ++j) {
+    A.load((s0 + j) * BK, ra[j]);
+    B.load((s0 + j) * BK, rb[j]);
+    __builtin_amdgcn_sched_barrier(0);  // in this order: the loop's waits count on it
+  }
   // step i's operands from registers i % AHEAD to image i % 2, and the registers on to step i + AHEAD
-  auto stage = [&](auto j_c, int i) {
+  typedef std::true_type More;
+  typedef std::false_type Last;
+  auto stage = [&](auto j_c, auto more, int i) {
     constexpr int j = decltype(j_c)::value;
     A.store(smem + (j & 1) * kStage, (s0 + i) * BK, ra[j]);
     B.store(smem + (j & 1) * kStage + OpA::kBytes, (s0 + i) * BK, rb[j]);
-    if (i + AHEAD < n) {
+    if constexpr (decltype(more)::value) {
       A.load((s0 + i + AHEAD) * BK, ra[j]);
       B.load((s0 + i + AHEAD) * BK, rb[j]);
     }
   };
-  if (n > 0) stage(std::integral_constant<int, 0>(), 0);
+  stage(std::integral_constant<int, 0>(), More(), 0);
   __syncthreads();
-  auto step = [&](auto j_c, int i) {
+  auto step = [&](auto j_c, auto more, int i) {
     constexpr int j = decltype(j_c)::value;
     const lds_t* cur = smem + (j & 1) * kStage;
     // the other image was read a step ago, before the last barrier
-    if (i + 1 < n) stage(std::integral_constant<int, (j + 1) % AHEAD>(), i + 1);
+    stage(std::integral_constant<int, (j + 1) % AHEAD>(), more, i + 1);
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       u32x4 fa[FM], fb[FN];
@@ -206,13 +211,19 @@ __global__ __launch_bounds__(NT) void linear_tile_kernel(LinearArgs p) {
     }
     __syncthreads();
   };
-  for (int i = 0; i < n; i += AHEAD) {
-    step(std::integral_constant<int, 0>(), i);
-    if (i + 1 < n) step(std::integral_constant<int, 1>(), i + 1);
+  int i = 0;
+  for (; i + AHEAD <= n; i += AHEAD) {  // one way through: a way out of its middle would count as skipped loads too
+    step(std::integral_constant<int, 0>(), More(), i);
+    step(std::integral_constant<int, 1>(), More(), i + 1);
     if constexpr (AHEAD > 2) {
-      if (i + 2 < n) step(std::integral_constant<int, 2>(), i + 2);
-      if (i + 3 < n) step(std::integral_constant<int, 3>(), i + 3);
+      step(std::integral_constant<int, 2>(), More(), i + 2);
+      step(std::integral_constant<int, 3>(), More(), i + 3);
     }
+  }
+  if (i < n) step(std::integral_constant<int, 0>(), Last(), i);
+  if constexpr (AHEAD > 2) {
+    if (i + 1 < n) step(std::integral_constant<int, 1>(), Last(), i + 1);
+    if (i + 2 < n) step(std::integral_constant<int, 2>(), Last(), i + 2);
   }
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
@@ -260,17 +271,17 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs p) {
   epilogue4(p.epi, m, n, p.N - n, p.vec != 0, v);
 }
 
-template <int B, bool ACOL, bool BCOL, int AHEAD = B == 64 ? 4 : 2>
+template <int BM, int BN, bool ACOL, bool BCOL, int AHEAD = BM + BN < 256 ? 4 : 2>
 int launch(const LinearArgs& p, hipStream_t st) {
-  const int64_t tiles = (int64_t)((p.M + B - 1) / B) * ((p.N + B - 1) / B);
+  const int64_t tiles = (int64_t)((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
   if (tiles >= (1LL << 31)) return -2;
   const dim3 grid((unsigned)tiles, (unsigned)p.splits);
   if (p.vec) {
-    if (p.epi.f16) linear_tile_kernel<B, B, AHEAD, ACOL, BCOL, true, true><<<grid, NT, 0, st>>>(p);
-    else linear_tile_kernel<B, B, AHEAD, ACOL, BCOL, true, false><<<grid, NT, 0, st>>>(p);
-  } else if constexpr (B == 64) {
-    if (p.epi.f16) linear_tile_kernel<B, B, AHEAD, ACOL, BCOL, false, true><<<grid, NT, 0, st>>>(p);
-    else linear_tile_kernel<B, B, AHEAD, ACOL, BCOL, false, false><<<grid, NT, 0, st>>>(p);
+    if (p.epi.f16) linear_tile_kernel<BM, BN, AHEAD, ACOL, BCOL, true, true><<<grid, NT, 0, st>>>(p);
+    else linear_tile_kernel<BM, BN, AHEAD, ACOL, BCOL, true, false><<<grid, NT, 0, st>>>(p);
+  } else if constexpr (BM + BN == 128) {
+    if (p.epi.f16) linear_tile_kernel<BM, BN, AHEAD, ACOL, BCOL, false, true><<<grid, NT, 0, st>>>(p);
+    else linear_tile_kernel<BM, BN, AHEAD, ACOL, BCOL, false, false><<<grid, NT, 0, st>>>(p);
   }
   if (p.splits > 1) {
     const hipError_t e = hipGetLastError();
@@ -282,18 +293,36 @@ int launch(const LinearArgs& p, hipStream_t st) {
   return (int)hipGetLastError();
 }
 
-// Tile edge and splits of a product.  Measured, us (forward, bias and GELU in brackets): splitting 256 tiles
-// costs where k is short -- 2048 x 512 x 2048 15 (23) whole, 26 (28) in two; 1024^3 10 (12) and 15 (17) --
-// and pays where it is long: 1000 x 4096 x 1000 30 (32) and 25 (25); 128 x 4096 x 4096, 128 tiles in four, 17.
+// Tile and splits of a product.  Measured, us, in 64 x 64 / 64 x 128 / 128 x 128 tiles:
+//   y with bias and GELU: 2048 x 1536 x 2048 29 / 29 / 34, 3000 x 1024 x 3000 45 / 49 / 53, 4096 x 1024 x 4096
+//     75 / 75 / 67 (a small tile's epilogue hides behind the other tiles of its CU);
+//   dx: 2048 x 2304 x 768 23 / 21 / 30, 2048 x 2048 x 512 15 / 19 / 28, 2048^3 38 / 30 / 29;
+//   dW: 2304 x 2048 x 768 27 / 23 / 29, 2048 x 2048 x 512 19 / 23 / 29, 2048^3 48 / 33 / 31.
+// Splits (64 x 64; one, two, four): 512 x 4096 x 1024 21 / 16 / 17, 1000 x 4096 x 1000 22 / 24 / 26, 512 x 1024 x
+// 1024 8 / 10 / 13; dW 768 x 4096 x 768 32 / 30 / 25 (three: 23), 256 x 2048 x 256 18 / 13 / 11.
 struct Plan {
-  int tile, splits;
+  int bm, bn, splits;
 };
-Plan plan(int M, int N, int K, int vec) {
-  auto tiles = [&](int b) { return (int64_t)((M + b - 1) / b) * ((N + b - 1) / b); };
+Plan plan(int M, int N, int K, int vec, int acol, int bcol) {
+  auto tiles = [&](int bm, int bn) { return (int64_t)((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
+  Plan r{64, 64, 1};
+  if (vec) {  // shifted loads leave larger tiles no registers
+    if (tiles(128, 128) >= (bcol ? 192 : 768)) r.bm = r.bn = 128;
+    else if (bcol && tiles(64, 64) > 256) r.bn = 128;
+  }
+  // The time in us but for what every plan has: a step of a 64 x 64 tile takes 0.27 (0.42 with a transposed A, 0.8
+  // with shifted loads), several tiles on a CU 0.85 (0.6) of their sum, the second kernel 3 and its sums at 4 TB/s.
   const int steps = (K + BK - 1) / BK;
-  Plan r{vec && tiles(128) >= 256 ? 128 : 64, 1};  // shifted loads leave 128 x 128 no registers for two a SIMD
-  const int64_t t = tiles(r.tile);
-  if (steps >= 8 && (t < 256 || (t < 512 && steps >= 48))) r.splits = (int)std::min<int64_t>({(512 + t - 1) / t, steps / 4, 32});
+  const double more = vec ? 0.85 : 0.6, step = (!vec ? 0.8 : acol ? 0.42 : 0.27) * r.bm * r.bn / 4096.0 * (r.bm + r.bn > 128 ? 0.75 : 1.0);
+  double best = 1e30;
+  for (int s = 1; s <= 32 && (s == 1 || steps / s >= 4); ++s) {
+    const double rounds = (double)((tiles(r.bm, r.bn) * s + 255) / 256);
+    const double us = (steps + s - 1) / s * step * std::max(1.0, more * rounds) + (s > 1 ? 3.0 + 2e-6 * s * M * N : 0.0);
+    if (us < best) {
+      best = us;
+      r.splits = s;
+    }
+  }
   return r;
 }
 
@@ -301,13 +330,13 @@ Plan plan(int M, int N, int K, int vec) {
 
 extern "C" {
 
-// The time that a product takes here at the usual 500 TF/s, in us (measured: 525 at 2048^3, 640 at 4096 x
-// 1024 x 4096, 850 where there are tiles for many rounds; the wide kernel is the faster one there).
+// The time that a product takes here at the usual 500 TF/s, in us (measured: 520 at 2048^3, 670 at 4096 x
+// 1024 x 4096, 930 where there are tiles for many rounds; the wide kernel is the faster one there).
 double st_linear_tile_us(int M, int N, int K) { return 4.0 + 2.0 * M * N * K / 5e8; }
 
 // fp32 workspace elements of a product.
-int64_t st_linear_tile_ws(int M, int N, int K, int vec) {
-  const Plan r = plan(M, N, K, vec);
+int64_t st_linear_tile_ws(int M, int N, int K, int vec, int acol, int bcol) {
+  const Plan r = plan(M, N, K, vec, acol, bcol);
   return r.splits > 1 ? (int64_t)r.splits * M * N : 0;
 }
 
@@ -315,15 +344,13 @@ int64_t st_linear_tile_ws(int M, int N, int K, int vec) {
 // floats.  -2: outside the kernel's.
 int st_linear_tile(LinearArgs* p, int acol, int bcol, hipStream_t st) {
   if (p->M <= 0 || p->N <= 0 || p->K <= 0 || (acol && !bcol)) return -2;
-  const Plan r = plan(p->M, p->N, p->K, p->vec);
+  const Plan r = plan(p->M, p->N, p->K, p->vec, acol, bcol);
   p->splits = r.splits;
   if (r.splits > 1 && !p->ws) return -2;
-  if (r.tile == 128) {
-    if (!bcol) return launch<128, false, false>(*p, st);
-    return acol ? launch<128, true, true>(*p, st) : launch<128, false, true>(*p, st);
-  }
-  if (!bcol) return launch<64, false, false>(*p, st);
-  return acol ? launch<64, true, true>(*p, st) : launch<64, false, true>(*p, st);
+  if (!bcol) return r.bm == 128 ? launch<128, 128, false, false>(*p, st) : launch<64, 64, false, false>(*p, st);
+  if (r.bm == 128) return acol ? launch<128, 128, true, true>(*p, st) : launch<128, 128, false, true>(*p, st);
+  if (r.bn == 128) return acol ? launch<64, 128, true, true>(*p, st) : launch<64, 128, false, true>(*p, st);
+  return acol ? launch<64, 64, true, true>(*p, st) : launch<64, 64, false, true>(*p, st);
 }
 
 }  // extern "C"

@@ -80,6 +80,8 @@ SHAPES = [(1, 8, 4), (1, 1, 1), (3, 33, 7), (16, 256, 128), (17, 1000, 264), (33
 # products that the 256 x 256 tiles take: whole and cut tiles, ragged edges, one step of k, several rounds
 WIDE = [(512, 256, 512), (1025, 320, 776), (777, 1024, 264)]
 LARGE = [(4096, 512, 4104), (2056, 2048, 2568), (8200, 64, 8192), (16448, 1280, 1288), (300, 8192, 1024)]
+# the smaller tiles, each in turn: 128 x 128 in y, 64 x 128 in dx, in dW, in dW with k split, 128 x 128 in dx, in dW
+TILES = [(4104, 136, 3080), (2056, 776, 520), (520, 776, 2312), (4104, 776, 1352), (2056, 1544, 328), (328, 1544, 2056)]
 
 
 @pytest.mark.parametrize("device", DEVICES)
@@ -92,7 +94,7 @@ def test_shapes(device, dtype, m, k, n):
 @pytest.mark.gpu
 @pytest.mark.parametrize("act,residual,rdtype,dtype", [("gelu", True, torch.float32, torch.bfloat16), ("none", True, None, torch.float16),
                                                        ("silu", True, None, torch.bfloat16), ("gelu_tanh", False, None, torch.bfloat16)])
-@pytest.mark.parametrize("m,k,n", LARGE)
+@pytest.mark.parametrize("m,k,n", LARGE + TILES)
 def test_large(m, k, n, act, residual, rdtype, dtype):
     """Against fp32 products on the GPU (the library's, checked at 64 bits where that is quick), whole tensors."""
     c = _inputs("cuda", m, k, n, dtype, True, residual, rdtype, seed=m)
