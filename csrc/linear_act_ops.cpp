@@ -14,7 +14,7 @@ using st::LinearArgs;
 extern "C" {
 int64_t st_linear_tile_ws(int M, int N, int K, int vec, int acol, int bcol);
 int st_linear_tile(LinearArgs* p, int acol, int bcol, hipStream_t st);
-double st_linear_tile_us(int M, int N, int K);
+double st_linear_tile_us(int M, int N, int K, int vec, int acol, int bcol);
 int st_linear_rows(const LinearArgs* p, hipStream_t st);
 int64_t st_linear_wide_ws(const LinearArgs* p);
 double st_linear_wide_us(const LinearArgs* p, int acol, int bcol);
@@ -73,11 +73,13 @@ void product(const at::Tensor& A, bool acol, const at::Tensor& B, bool bcol, st:
   p.vec = vec && (p.lda * 128 + K) * 2 < most && (p.ldb * 128 + K) * 2 < most && ca % 8 == 0 && cb % 8 == 0 &&
           N % 4 == 0 && p.lda % 8 == 0 && p.ldb % 8 == 0 && aligned(A) && aligned(B);
   int rc = -2;
-  // few rows stream the weight; else whichever tiling is expected to be faster
+  // few rows stream the weight; else whichever tiling is expected to be faster.  Measured, us, smaller tiles / 256 x
+  // 256: y with GELU 8192 x 1024 x 1024 41 / 47, 8192 x 1280 x 1280 57 / 52, 4096 x 1024 x 4096 67 / 52; dx 4096 x
+  // 4096 x 1024 50 / 66, 24576 x 1280 x 1280 107 / 98; dW 4096 x 4096 x 1024 51 / 68, 1280 x 24576 x 1280 137 / 99.
   if (!acol && !bcol && M <= 64) rc = st_linear_rows(&p, stream());
   if (rc == -2) {
     const double wide = st_linear_wide_us(&p, acol, bcol);
-    const bool use_wide = wide >= 0.0 && wide < st_linear_tile_us(p.M, p.N, p.K);
+    const bool use_wide = wide >= 0.0 && wide < st_linear_tile_us(p.M, p.N, p.K, p.vec, acol, bcol);
     at::Tensor ws;
     if (const int64_t n = use_wide ? st_linear_wide_ws(&p) : st_linear_tile_ws(p.M, p.N, p.K, p.vec, acol, bcol)) {
       ws = at::empty({n}, A.options().dtype(at::kFloat));

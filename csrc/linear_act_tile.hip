@@ -302,24 +302,27 @@ int launch(const LinearArgs& p, hipStream_t st) {
 // 1024 8 / 10 / 13; dW 768 x 4096 x 768 32 / 30 / 25 (three: 23), 256 x 2048 x 256 18 / 13 / 11.
 struct Plan {
   int bm, bn, splits;
+  double us;  // the time to expect
 };
 Plan plan(int M, int N, int K, int vec, int acol, int bcol) {
   auto tiles = [&](int bm, int bn) { return (int64_t)((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
-  Plan r{64, 64, 1};
+  Plan r{64, 64, 1, 1e30};
   if (vec) {  // shifted loads leave larger tiles no registers
     if (tiles(128, 128) >= (bcol ? 192 : 768)) r.bm = r.bn = 128;
     else if (bcol && tiles(64, 64) > 256) r.bn = 128;
   }
-  // The time in us but for what every plan has: a step of a 64 x 64 tile takes 0.27 (0.42 with a transposed A, 0.8
-  // with shifted loads), several tiles on a CU 0.85 (0.6) of their sum, the second kernel 3 and its sums at 4 TB/s.
+  // us of a step: 64 x 64 0.27 (0.42 with a transposed A, 0.8 with shifted loads), 64 x 128 0.5, 128 x 128 0.8;
+  // several tiles on a CU take 0.85 (0.6) of their sum, epilogues of 128 x 128 2 a round, the second kernel 3 and
+  // its sums at 4 TB/s.
   const int steps = (K + BK - 1) / BK;
-  const double more = vec ? 0.85 : 0.6, step = (!vec ? 0.8 : acol ? 0.42 : 0.27) * r.bm * r.bn / 4096.0 * (r.bm + r.bn > 128 ? 0.75 : 1.0);
-  double best = 1e30;
+  const double more = vec ? 0.85 : 0.6;
+  const double step = !vec || r.bm == 128 ? 0.8 : r.bn == 128 ? 0.5 : acol ? 0.42 : 0.27;
   for (int s = 1; s <= 32 && (s == 1 || steps / s >= 4); ++s) {
     const double rounds = (double)((tiles(r.bm, r.bn) * s + 255) / 256);
-    const double us = (steps + s - 1) / s * step * std::max(1.0, more * rounds) + (s > 1 ? 3.0 + 2e-6 * s * M * N : 0.0);
-    if (us < best) {
-      best = us;
+    const double us = 4.0 + (steps + s - 1) / s * step * std::max(1.0, more * rounds) +
+                      (r.bm == 128 && !bcol ? 2.0 * rounds : 0.0) + (s > 1 ? 3.0 + 2e-6 * s * M * N : 0.0);
+    if (us < r.us) {
+      r.us = us;
       r.splits = s;
     }
   }
@@ -330,9 +333,8 @@ Plan plan(int M, int N, int K, int vec, int acol, int bcol) {
 
 extern "C" {
 
-// The time that a product takes here at the usual 500 TF/s, in us (measured: 520 at 2048^3, 670 at 4096 x
-// 1024 x 4096, 930 where there are tiles for many rounds; the wide kernel is the faster one there).
-double st_linear_tile_us(int M, int N, int K) { return 4.0 + 2.0 * M * N * K / 5e8; }
+// The time in us that a product is expected to take here.
+double st_linear_tile_us(int M, int N, int K, int vec, int acol, int bcol) { return plan(M, N, K, vec, acol, bcol).us; }
 
 // fp32 workspace elements of a product.
 int64_t st_linear_tile_ws(int M, int N, int K, int vec, int acol, int bcol) {

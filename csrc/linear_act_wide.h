@@ -449,7 +449,8 @@ int cu_count() {
 
 // Tiles that are done whole, the parts that each of the others is cut into, and the time to expect.
 // Measured: a step of a tile takes some 1.6 us (24576 x 4096 x 14336), a round's epilogue 8, or 13 where
-// it writes fp32 parts; the second kernel reads those at some 4 TB/s and costs 6 us more.
+// it writes fp32 parts, the way to the first step 7; the second kernel reads the parts at some 4 TB/s and
+// costs 6 us more.
 constexpr int kGroup = 4;
 struct WidePlan {
   int nfull, splits;
@@ -458,10 +459,10 @@ struct WidePlan {
 WidePlan linear_wide_plan(int M, int N, int K) {
   const int cus = cu_count(), KT = (K + BK - 1) / BK;
   const int nv = ((M + BT - 1) / BT) * ((N + BT - 1) / BT), tail = nv % cus, rounds = (nv + cus - 1) / cus;
-  WidePlan best{nv, 1, rounds * (8.0 + 1.6 * KT)};
+  WidePlan best{nv, 1, 7.0 + rounds * (8.0 + 1.6 * KT)};
   for (int s = 2; tail && s <= 8 && KT / s >= 4; ++s) {
     const int parts = (tail * s + cus - 1) / cus;
-    const double us = (rounds - 1) * (8.0 + 1.6 * KT) + parts * (13.0 + 1.6 * ((KT + s - 1) / s)) + 6.0 + tail * s * 0.2621 / 4.0;
+    const double us = 7.0 + (rounds - 1) * (8.0 + 1.6 * KT) + parts * (13.0 + 1.6 * ((KT + s - 1) / s)) + 6.0 + tail * s * 0.2621 / 4.0;
     if (us < best.us) best = WidePlan{nv - tail, s, us};
   }
   return best;

@@ -77,9 +77,11 @@ def _compare(c, act):
 
 SHAPES = [(1, 8, 4), (1, 1, 1), (3, 33, 7), (16, 256, 128), (17, 1000, 264), (33, 72, 40), (64, 520, 1000), (65, 64, 64),
           (65, 65, 65), (130, 1000, 200), (300, 136, 8), (257, 100, 333), (129, 24, 2048), (1000, 520, 264)]
-# products that the 256 x 256 tiles take: whole and cut tiles, ragged edges, one step of k, several rounds
+# a few more rows, inner sizes of whole steps
 WIDE = [(512, 256, 512), (1025, 320, 776), (777, 1024, 264)]
 LARGE = [(4096, 512, 4104), (2056, 2048, 2568), (8200, 64, 8192), (16448, 1280, 1288), (300, 8192, 1024)]
+# the 256 x 256 tiles: one, two and three steps of k, cut tiles in y, dx and dW, whole ones of ragged edges
+LARGE += [(5128, 64, 8712), (3336, 128, 8456), (1288, 192, 8968), (4200, 1984, 4104), (6001, 1320, 5120), (4100, 1024, 4096), (5000, 1288, 5056)]
 # the smaller tiles, each in turn: 128 x 128 in y, 64 x 128 in dx, in dW, in dW with k split, 128 x 128 in dx, in dW
 TILES = [(4104, 136, 3080), (2056, 776, 520), (520, 776, 2312), (4104, 776, 1352), (2056, 1544, 328), (328, 1544, 2056)]
 
