@@ -10,6 +10,7 @@
 #include <algorithm>
 
 #include "block_norm_args.h"
+#include "capture_check.h"
 
 using st::NormArgs;
 
@@ -306,6 +307,8 @@ std::tuple<at::Tensor, at::Tensor> block_norm_autograd(const at::Tensor& h, cons
   check_call(h, residual, w1, b1, w2, b2);
   const bool same = stream_is_h(residual, gate, w1, scale);
   if (same && !has(w2)) return {at::Tensor(), h};
+  auto ptr = [](const opt& t) { return has(t) ? &*t : nullptr; };
+  st::check_capture({&h, ptr(residual), ptr(gate), ptr(w1), ptr(b1), ptr(w2), ptr(b2)}, "block_norm");
   auto r = BlockNorm::apply(h.contiguous(), rows_of(residual), rows_of(gate), rows_of(w1), rows_of(b1), rows_of(w2),
                             rows_of(b2), layer, scale, eps, !same);
   at::Tensor y = has(w2) ? r[0] : at::Tensor();

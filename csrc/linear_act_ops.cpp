@@ -7,6 +7,7 @@
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <hip/hip_runtime.h>
 
+#include "capture_check.h"
 #include "linear_act_args.h"
 
 using st::LinearArgs;
@@ -239,6 +240,10 @@ at::Tensor linear_act(const at::Tensor& x, const at::Tensor& w, const opt& bias,
   return std::get<0>(linear_act_fwd(x, w, bias, residual, act, false));
 }
 
+void check_capture(at::TensorList inputs) {
+  for (const auto& t : inputs) st::check_capture({&t}, "training call");
+}
+
 at::Tensor linear_act_autograd(const at::Tensor& x, const at::Tensor& w, const opt& bias, const opt& residual,
                                int64_t act) {
   const bool grad = x.requires_grad() || w.requires_grad() || (has(bias) && bias->requires_grad()) ||
@@ -247,6 +252,7 @@ at::Tensor linear_act_autograd(const at::Tensor& x, const at::Tensor& w, const o
     at::AutoDispatchBelowADInplaceOrView below;
     return linear_act(x, w, bias, residual, act);
   }
+  st::check_capture({&x, &w, has(bias) ? &*bias : nullptr, has(residual) ? &*residual : nullptr}, "linear_act");
   return LinearAct::apply(x, w, bias, residual, act);
 }
 
@@ -258,6 +264,7 @@ TORCH_LIBRARY_FRAGMENT(st_amd, m) {
   m.def("linear_act_dz(Tensor dy, Tensor? z, ScalarType type, int act, bool want_db, bool db_f32) -> (Tensor, Tensor)");
   m.def("linear_act_dx(Tensor dz, Tensor weight) -> Tensor");
   m.def("linear_act_dw(Tensor dz, Tensor x) -> Tensor");
+  m.def("check_capture(Tensor[] inputs) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(st_amd, CUDA, m) {
@@ -266,6 +273,7 @@ TORCH_LIBRARY_IMPL(st_amd, CUDA, m) {
   m.impl("linear_act_dz", &linear_act_dz);
   m.impl("linear_act_dx", &linear_act_dx);
   m.impl("linear_act_dw", &linear_act_dw);
+  m.impl("check_capture", &check_capture);
 }
 
 TORCH_LIBRARY_IMPL(st_amd, AutogradCUDA, m) { m.impl("linear_act", &linear_act_autograd); }

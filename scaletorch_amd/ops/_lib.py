@@ -69,6 +69,13 @@ def ops():
     return torch.ops.st_amd
 
 
+def check_capture(*inputs: torch.Tensor | None) -> None:
+    """Refuses a training call under graph capture whose gradients would be accumulated on another
+    stream, that of an earlier autograd graph still held (csrc/capture_check.h)."""
+    if torch.is_grad_enabled() and torch.cuda.is_current_stream_capturing():
+        ops().check_capture([t for t in inputs if t is not None])
+
+
 def load_error() -> str | None:
     return _load_error
 

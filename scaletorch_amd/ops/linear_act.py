@@ -11,7 +11,6 @@ of long sums, and x's type is what the matrix instructions take.
 """
 from __future__ import annotations
 
-
 import math
 
 import torch
@@ -107,5 +106,6 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
         t = torch.get_autocast_dtype("cuda")
         x, weight, bias = (v if v is None else v.to(t) for v in (x, weight, bias))
     if getattr(weight, "main_grad", None) is not None or getattr(bias, "main_grad", None) is not None:
+        _lib.check_capture(x, weight, bias, residual)
         return _LinearActFn.apply(x, weight, bias, residual, act)
     return _lib.ops().linear_act.default(x, weight, bias, residual, act)

@@ -370,3 +370,27 @@ def test_main_grad_takes_the_sums():
         assert ts[k].grad is None
         err = (ts[k].main_grad.double().cpu() - 2.0 - rg[k]).norm() / rg[k].norm()
         assert err <= 1e-5, k  # fp32 sums: no 16-bit rounding enters
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("main_grad", [False, True])
+def test_capture_beside_a_live_graph_is_refused(main_grad):
+    """Refused before anything of it is recorded; without the earlier graph the same capture works."""
+    h = torch.nn.Parameter(torch.randn(8, 64, device="cuda"))
+    w = torch.nn.Parameter(torch.ones(64, device="cuda"))
+    if main_grad:
+        w.main_grad = torch.zeros(64, device="cuda")
+    live = ops.block_norm(h, pre_weight=w)
+    for _ in range(2):
+        torch.cuda.synchronize()
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            keep = torch.zeros(4, device="cuda")
+            with torch.no_grad():
+                y = ops.block_norm(h, pre_weight=w)
+            if live is not None:
+                with pytest.raises(RuntimeError, match="earlier autograd graph"):
+                    ops.block_norm(h, pre_weight=w)
+            else:
+                torch.autograd.grad(ops.block_norm(h, pre_weight=w)[0], [h], torch.ones_like(h))
+        live = None
+    del keep, y

@@ -378,3 +378,27 @@ def test_autocast_casts_as_linear_does():
     assert torch.equal(y, want)
     dx, dw = torch.autograd.grad(y, (x, w), c["dy"])
     assert dx.dtype == torch.float32 and torch.equal(dx, g["x"].float()) and torch.equal(dw, g["w"].float())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("main_grad", [False, True])
+def test_capture_beside_a_live_graph_is_refused(main_grad):
+    """Refused before anything of it is recorded; without the earlier graph the same capture works."""
+    c = _inputs("cuda", 64, 64, 64, torch.bfloat16)
+    x, w = (torch.nn.Parameter(c[k]) for k in "xw")
+    if main_grad:
+        w.main_grad = torch.zeros(64, 64, device="cuda")
+    live = ops.linear_act(x, w, activation="gelu")
+    for _ in range(2):
+        torch.cuda.synchronize()
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            keep = torch.zeros(4, device="cuda")
+            with torch.no_grad():
+                y = ops.linear_act(x, w, activation="gelu")
+            if live is not None:
+                with pytest.raises(RuntimeError, match="earlier autograd graph"):
+                    ops.linear_act(x, w, activation="gelu")
+            else:
+                torch.autograd.grad(ops.linear_act(x, w, activation="gelu"), [x], c["dy"])
+        live = None
+    del keep, y
