@@ -26,8 +26,8 @@
 //
 // Measured, bf16, 24576 x 4096 x 14336 (2.89 TFLOP; the library's plain products in brackets): y alone 2.33
 // ms (1.87-1.95), with bias, GELU and z 2.45-2.55, with tanh GELU, z and residual 2.63-2.77; dx 2.16-2.18
-// (2.12-2.17); dW 2.26-2.36 (2.91-2.93), of it 26-39 us for the cut tiles.  8192 x 1280 x 5120: y with GELU and z 159-165
-// us (115-116 plain), dx 121-124 (102-106), dW 131-137 (116-124).  The chip holds its power limit here:
+// (2.12-2.17); dW 2.26-2.34 (2.91-2.93), of it some 16 us for the cut tiles.  8192 x 1280 x 5120: y with GELU and z 159-165
+// us (115-116 plain), dx 117-121 (102-106), dW 117 (116-124).  The chip holds its power limit here:
 // the library's kernel keeps the matrix units 86 % busy at 1.66 GHz, this one 62 % at 1.85 and 49 %
 // (epilogues) at 2.1, with no LDS conflicts and 16 % of the time in waits.  Lost to this schedule: both
 // regions released at MFMA 40 and publication at 96 (1-3 % slower), copies three MFMAs apart (6 %),
@@ -415,6 +415,9 @@ __global__ __launch_bounds__(NT, 1) void linear_wide_kernel(LinearArgs p, int gm
 #pragma clang diagnostic pop
 
 // The parts of the cut tiles, in order, then their epilogue: an (i, j) block of a tile a workgroup.
+// Neighbouring 16 x 16 blocks of a workgroup: it then writes whole 128-byte lines.  100 tiles of two parts (52 MB)
+// take 13 us; with one block each, whose lines belong to several XCDs, 27.
+constexpr int kJoin = 4;
 __global__ __launch_bounds__(NT) void linear_wide_join_kernel(LinearArgs p, int gm, int nfull) {
   const int nbm = (p.M + BT - 1) / BT, nbn = (p.N + BT - 1) / BT, nv = nbm * nbn, tail = nv - nfull;
   const int id = xcd_remap(nfull + (int)blockIdx.x, nv), per = gm * nbn, grp = id / per, in = id % per;
@@ -422,17 +425,22 @@ __global__ __launch_bounds__(NT) void linear_wide_join_kernel(LinearArgs p, int 
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
   const int m0 = (grp * gm + in % gsz) * BT + (wid >> 1) * 128 + (lane & 15);
   const int n0 = (in / gsz) * BT + (wid & 1) * 128 + 4 * (lane >> 4);
-  const int ij = (int)blockIdx.y, m = m0 + 16 * (ij >> 3), n = n0 + 16 * (ij & 7);
+  const int ij = (int)blockIdx.y * kJoin, m = m0 + 16 * (ij >> 3), n = n0 + 16 * (ij & 7);
   const f32x4* w = reinterpret_cast<const f32x4*>(p.ws) + (int64_t)blockIdx.x * (BT * BT / 4) + ij * NT + threadIdx.x;
-  f32x4 part[8];  // all requested before the first sum
+  f32x4 part[8][kJoin];  // all requested before the first sum
 #pragma unroll
   for (int s = 0; s < 8; ++s)
-    if (s < p.splits) part[s] = w[(int64_t)s * tail * (BT * BT / 4)];
-  f32x4 v = part[0];
+    if (s < p.splits)
 #pragma unroll
-  for (int s = 1; s < 8; ++s)
-    if (s < p.splits) v += part[s];
-  if (m < p.M && n < p.N) epilogue4(p.epi, m, n, p.N - n, true, v);
+      for (int j = 0; j < kJoin; ++j) part[s][j] = w[(int64_t)s * tail * (BT * BT / 4) + j * NT];
+#pragma unroll
+  for (int j = 0; j < kJoin; ++j) {
+    f32x4 v = part[0][j];
+#pragma unroll
+    for (int s = 1; s < 8; ++s)
+      if (s < p.splits) v += part[s][j];
+    if (m < p.M && n + 16 * j < p.N) epilogue4(p.epi, m, n + 16 * j, p.N - n - 16 * j, true, v);
+  }
 }
 
 int cu_count() {
@@ -481,7 +489,7 @@ int launch(const LinearArgs& p, hipStream_t st) {
   if (w.splits > 1) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
-    linear_wide_join_kernel<<<dim3((unsigned)(nv - w.nfull), 64), NT, 0, st>>>(q, kGroup, w.nfull);
+    linear_wide_join_kernel<<<dim3((unsigned)(nv - w.nfull), 64 / kJoin), NT, 0, st>>>(q, kGroup, w.nfull);
   }
   return (int)hipGetLastError();
 }
