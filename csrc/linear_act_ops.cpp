@@ -74,10 +74,12 @@ void product(const at::Tensor& A, bool acol, const at::Tensor& B, bool bcol, st:
   p.vec = vec && (p.lda * 128 + K) * 2 < most && (p.ldb * 128 + K) * 2 < most && ca % 8 == 0 && cb % 8 == 0 &&
           N % 4 == 0 && p.lda % 8 == 0 && p.ldb % 8 == 0 && aligned(A) && aligned(B);
   int rc = -2;
-  // few rows stream the weight; else whichever tiling is expected to be faster.  Measured, us, smaller tiles / 256 x
-  // 256: y with GELU 8192 x 1024 x 1024 41 / 47, 8192 x 1280 x 1280 57 / 52, 4096 x 1024 x 4096 67 / 52; dx 4096 x
-  // 4096 x 1024 50 / 66, 24576 x 1280 x 1280 107 / 98; dW 4096 x 4096 x 1024 51 / 68, 1280 x 24576 x 1280 137 / 99.
-  if (!acol && !bcol && M <= 64) rc = st_linear_rows(&p, stream());
+  // Few rows stream the weight.  Measured, us, streamed / tiles: 4096 -> 14336 4 rows 27 / 25 (from memory 27 / 31),
+  // 8 rows 28 / 21; 14336 -> 4096 8 rows 29 / 25; but 4096 -> 4096 8 rows 10 / 12, 16 rows 11 / 12; 1280 -> 5120 8 / 10.
+  // Else whichever tiling is expected to be faster: smaller tiles / 256 x 256: y with GELU 8192 x 1024 x 1024 41 / 47,
+  // 8192 x 1280 x 1280 57 / 52, 4096 x 1024 x 4096 67 / 52; dx 4096 x 4096 x 1024 50 / 66, 24576 x 1280 x 1280 107 / 98;
+  // dW 4096 x 4096 x 1024 51 / 68, 1280 x 24576 x 1280 137 / 99.
+  if (!acol && !bcol && (M <= 4 || (M <= 16 && N * K <= 1 << 24))) rc = st_linear_rows(&p, stream());
   if (rc == -2) {
     const double wide = st_linear_wide_us(&p, acol, bcol);
     const bool use_wide = wide >= 0.0 && wide < st_linear_tile_us(p.M, p.N, p.K, p.vec, acol, bcol);

@@ -77,6 +77,8 @@ def _compare(c, act):
 
 SHAPES = [(1, 8, 4), (1, 1, 1), (3, 33, 7), (16, 256, 128), (17, 1000, 264), (33, 72, 40), (64, 520, 1000), (65, 64, 64),
           (65, 65, 65), (130, 1000, 200), (300, 136, 8), (257, 100, 333), (129, 24, 2048), (1000, 520, 264)]
+# few rows: 16 and 32 columns a workgroup, ends of k and of the columns inside one
+SHAPES += [(2, 40, 24), (4, 72, 8200), (5, 1000, 264), (9, 2056, 1000), (16, 1032, 8200)]
 # a few more rows, inner sizes of whole steps
 WIDE = [(512, 256, 512), (1025, 320, 776), (777, 1024, 264)]
 LARGE = [(4096, 512, 4104), (2056, 2048, 2568), (8200, 64, 8192), (16448, 1280, 1288), (300, 8192, 1024)]
