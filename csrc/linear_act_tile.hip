@@ -1,18 +1,19 @@
 // The product with its epilogue for every shape: BM x BN tiles, 2 x 2 waves, k in steps of 64.
 //
-// A step's operands go global -> registers (16-byte loads, or element by element where rows are not
-// aligned), issued several steps ahead (a step of a small tile computes for 0.1 us, a load takes one),
-// then to one of two LDS images, from which the waves read their MFMA fragments; one barrier a step.
-// kRow images are [rows][64 k], 16-byte chunk c of row r at c ^ ((r >> 1) & 7); kCol images [64 k][rows]
-// in 256-byte (64-column tiles: 128-byte) rows, read with the transposing LDS read, chunk c of row k at
-// c ^ swz(k).  Chunks behind an operand's end are zeros.  Few tiles: k is split over workgroups, whose fp32 sums a second kernel adds up in
-// order before the epilogue.
+// A step's operands go global -> registers (16-byte loads, from any element where rows are not aligned),
+// issued several steps ahead (a step of a small tile computes for 0.1 us, a load takes one), then to one of
+// two LDS images, from which the waves read their MFMA fragments; one barrier a step.  kRow images are
+// [rows][64 k], 16-byte chunk c of row r at c ^ ((r >> 1) & 7); kCol images [64 k][rows] in 256-byte
+// (64-column tiles: 128-byte) rows, read with the transposing LDS read, chunk c of row k at c ^ swz(k).
+// Chunks behind an operand's end are zeros.  Few tiles: k is split over workgroups, whose fp32 sums a second
+// kernel adds up in order before the epilogue.
 //
-// Bound by a step's chain (LDS writes, barrier, fragments: 0.27 us for a 64 x 64 tile alone on its CU, of it 0.06
-// of matrix instructions) where there are few tiles, by the L1s where several share a CU.  Measured, bf16: 2048^3 33 us (520 TF/s; the library's product 26), its
-// gradients 31 (28-30), 1024^3 9 us (the library's product 21-25), 777 x 1000 x 2504 with the epilogue 20 us
-// (22 alone), 777 x 1001 x 2503 25 us, 24576 x 4096 x 14336 3.1 ms (930 TF/s).  With loads that some paths skip
-// every fourth step of the loop waited for all of them: dx of 2048^3 took 33 us and not 29.
+// Bound by a step's chain (LDS writes, barrier, fragments: 0.27 us for a 64 x 64 tile alone on its CU, of it
+// 0.06 of matrix instructions) where there are few tiles, by the L1s where several share a CU.  Measured,
+// bf16: 2048^3 33 us (520 TF/s; the library's product 26), its gradients 31 (28-30), 1024^3 9 us (21-25),
+// 64 x 4096 x 14336 22 us (24), 777 x 1000 x 2504 with the epilogue 20 us (22 alone), 777 x 1001 x 2503 25 us,
+// 24576 x 4096 x 14336 3.1 ms (930 TF/s).  With loads that some paths skip every fourth step of the loop
+// waited for all of them: dx of 2048^3 took 33 us and not 29-31.
 #include <algorithm>
 #include <type_traits>
 
