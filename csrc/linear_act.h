@@ -21,7 +21,10 @@ typedef _Float16 hx8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 typedef __amdgpu_buffer_rsrc_t rsrc_t;
-constexpr uint32_t kOut = 0xffffffe0u;  // an offset behind every range: loads give zero, stores go nowhere
+// A lane's offset behind every range: loads give zero, stores go nowhere.  The range test subtracts the scalar
+// offset from the range's size in 32 bits: with a scalar offset of up to the size the difference stays below
+// 2^31 and kOut outside, with a larger one it can wrap to above kOut.  So scalar offsets stay inside the range.
+constexpr uint32_t kOut = 0xffffffe0u;
 ST_DEVICE uint32_t uni(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
 ST_DEVICE rsrc_t rsrc_of(const void* base, uint32_t bytes) {  // of wave-uniform values
   const uint64_t a = (uint64_t)base;

@@ -48,7 +48,7 @@ __global__ __launch_bounds__(256) void linear_rows_kernel(LinearArgs p) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const bool in = s + u < s1 && (s + u) * 32 + 8 * g < p.K;  // K % 8 == 0: the 8 are all in or all out
-      const int k2 = min(s + u, s1) * 64;
+      const int k2 = min(s + u, steps - 1) * 64;  // inside both ranges: a scalar offset past a range's end would wrap the test of kOut
 #pragma unroll
       for (int b = 0; b < NB; ++b)  // 2: non-temporal
         fw[h][u][b] = __builtin_amdgcn_raw_buffer_load_b128(rw, in ? ow[b] : kOut, k2, 2);

@@ -74,13 +74,13 @@ struct Operand {
   }
   ST_DEVICE void load(int k0, Regs& reg) const {
     if constexpr (VEC) {
-      const int most = min(R, rows);
+      const int most = min(R, rows), so = COL || k0 >= K ? 0 : k0 * 2;  // the scalar offset: inside the range, as kOut's test needs
       const rsrc_t rs = COL ? rsrc_of(base + (int64_t)k0 * ld, k0 < K ? (uint32_t)(((int64_t)(min(BK, K - k0) - 1) * ld + most) * 2) : 0u)
                             : rsrc_of(base, (uint32_t)(((int64_t)(most - 1) * ld + K) * 2));
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
         const uint32_t off = (uint32_t)(((COL ? (int64_t)k_of(i) * ld + row_of(i) : (int64_t)row_of(i) * ld + k_of(i)) * 2));
-        reg[i] = __builtin_amdgcn_raw_buffer_load_b128(rs, left(i, k0) > 0 ? off : kOut, COL ? 0 : k0 * 2, 0);
+        reg[i] = __builtin_amdgcn_raw_buffer_load_b128(rs, left(i, k0) > 0 ? off : kOut, so, 0);
       }
     } else {
 #pragma unroll

@@ -404,3 +404,12 @@ def test_capture_beside_a_live_graph_is_refused(main_grad):
                 torch.autograd.grad(ops.linear_act(x, w, activation="gelu"), [x], c["dy"])
         live = None
     del keep, y
+
+
+# one row of x behind whose last step of k only a part of a step is left (24 of 32, 56 of 64 values), and a last
+# tile of one row with the same end, in y and, of the columns, in dx
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("m,k,n", [(1, 24, 8), (1, 56, 24), (1, 88, 8200), (1, 4088, 64), (65, 56, 136), (65, 120, 136),
+                                   (129, 184, 264), (65, 64, 56), (193, 128, 184), (257, 1016, 2040)])
+def test_last_step_of_a_single_row(device, m, k, n):
+    _compare(_inputs(device, m, k, n, torch.bfloat16), "gelu")
