@@ -10,6 +10,7 @@
 #include <vector>
 
 #include "adamw_multi.h"
+#include "forward_grad_check.h"
 
 extern "C" int st_adamw_multi(const AdamTable* tab, int count, const AdamScalars* h, int gtype, int ptype, int eight,
                               hipStream_t st);
@@ -49,6 +50,8 @@ void adamw_multi_(at::TensorList params, at::TensorList grads, at::TensorList ex
               "adamw_multi: lists of different lengths");
   if (N == 0) return;
   TORCH_CHECK(step >= 1 && step <= UINT32_MAX, "adamw_multi: step counts from 1, got ", step);
+  for (const at::TensorList l : {params, grads, exp_avg, exp_avg_sq, masters, scales})
+    st::refuse_forward_grad(l, "adamw_multi");
   const auto dev = params[0].device();
   auto check = [&](const at::Tensor& t, int64_t n, const char* what, size_t i) {
     TORCH_CHECK(t.is_cuda() && t.device() == dev, "adamw_multi: ", what, " ", i, " must be on ", dev, ", got ",
@@ -58,6 +61,7 @@ void adamw_multi_(at::TensorList params, at::TensorList grads, at::TensorList ex
   };
   AdamScalars h{};
   if (clip_coef.has_value() && clip_coef->defined()) {
+    st::refuse_forward_grad(*clip_coef, "adamw_multi");
     check(*clip_coef, 1, "clip_coef", 0);
     TORCH_CHECK(clip_coef->scalar_type() == at::kFloat, "adamw_multi: clip_coef must be fp32");
     h.clip = clip_coef->data_ptr<float>();

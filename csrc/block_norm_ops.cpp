@@ -11,6 +11,7 @@
 
 #include "block_norm_args.h"
 #include "capture_check.h"
+#include "forward_grad_check.h"
 
 using st::NormArgs;
 
@@ -298,6 +299,8 @@ std::tuple<at::Tensor, at::Tensor> block_norm(const at::Tensor& h, const opt& re
 std::tuple<at::Tensor, at::Tensor> block_norm_autograd(const at::Tensor& h, const opt& residual, const opt& gate,
                                                        const opt& w1, const opt& b1, const opt& w2, const opt& b2,
                                                        bool layer, double scale, double eps) {
+  auto ptr = [](const opt& t) { return has(t) ? &*t : nullptr; };
+  st::refuse_forward_grad({&h, ptr(residual), ptr(gate), ptr(w1), ptr(b1), ptr(w2), ptr(b2)}, "block_norm");
   bool grad = h.requires_grad();
   for (const opt* t : {&residual, &gate, &w1, &b1, &w2, &b2}) grad |= has(*t) && (*t)->requires_grad();
   if (!grad || !at::GradMode::is_enabled()) {
@@ -307,7 +310,6 @@ std::tuple<at::Tensor, at::Tensor> block_norm_autograd(const at::Tensor& h, cons
   check_call(h, residual, w1, b1, w2, b2);
   const bool same = stream_is_h(residual, gate, w1, scale);
   if (same && !has(w2)) return {at::Tensor(), h};
-  auto ptr = [](const opt& t) { return has(t) ? &*t : nullptr; };
   st::check_capture({&h, ptr(residual), ptr(gate), ptr(w1), ptr(b1), ptr(w2), ptr(b2)}, "block_norm");
   auto r = BlockNorm::apply(h.contiguous(), rows_of(residual), rows_of(gate), rows_of(w1), rows_of(b1), rows_of(w2),
                             rows_of(b2), layer, scale, eps, !same);

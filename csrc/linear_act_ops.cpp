@@ -8,6 +8,7 @@
 #include <hip/hip_runtime.h>
 
 #include "capture_check.h"
+#include "forward_grad_check.h"
 #include "linear_act_args.h"
 
 using st::LinearArgs;
@@ -248,13 +249,15 @@ void check_capture(at::TensorList inputs) {
 
 at::Tensor linear_act_autograd(const at::Tensor& x, const at::Tensor& w, const opt& bias, const opt& residual,
                                int64_t act) {
+  auto ptr = [](const opt& t) { return has(t) ? &*t : nullptr; };
+  st::refuse_forward_grad({&x, &w, ptr(bias), ptr(residual)}, "linear_act");
   const bool grad = x.requires_grad() || w.requires_grad() || (has(bias) && bias->requires_grad()) ||
                     (has(residual) && residual->requires_grad());
   if (!grad || !at::GradMode::is_enabled()) {
     at::AutoDispatchBelowADInplaceOrView below;
     return linear_act(x, w, bias, residual, act);
   }
-  st::check_capture({&x, &w, has(bias) ? &*bias : nullptr, has(residual) ? &*residual : nullptr}, "linear_act");
+  st::check_capture({&x, &w, ptr(bias), ptr(residual)}, "linear_act");
   return LinearAct::apply(x, w, bias, residual, act);
 }
 

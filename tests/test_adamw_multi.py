@@ -428,3 +428,22 @@ def test_offsets_past_32_bits():
         assert torch.allclose(c["params"][0][s], torch.tensor(0.75, device="cuda"), atol=1e-6)
         assert (c["exp_avg"][0][s].float() == 448).all() and (c["exp_avg_sq"][0][s].float() == 448).all()
     assert (c["scales"][0][-3:] > 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["params", "grads", "exp_avg", "exp_avg_sq", "clip_coef"])
+def test_forward_mode_is_refused(which):
+    """The update of a tangent is not implemented; nothing is written by the refused call."""
+    import torch.autograd.forward_ad as fwd
+
+    c = _case([(300,)], "cuda")
+    before, clip = _clone(c), torch.ones(1, device="cuda")
+    with fwd.dual_level():
+        d = {k: list(v) for k, v in c.items()}
+        if which == "clip_coef":
+            clip = fwd.make_dual(clip, torch.ones_like(clip))
+        else:
+            d[which][0] = fwd.make_dual(d[which][0], torch.ones(300, device="cuda"))
+        with pytest.raises(NotImplementedError):
+            ops.adamw_multi_(**d, step=1, lr=1e-3, clip_coef=clip)
+    assert all(torch.equal(a, b) for k in ("params", "exp_avg", "exp_avg_sq") for a, b in zip(c[k], before[k]))

@@ -394,3 +394,36 @@ def test_capture_beside_a_live_graph_is_refused(main_grad):
                 torch.autograd.grad(ops.block_norm(h, pre_weight=w)[0], [h], torch.ones_like(h))
         live = None
     del keep, y
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("which", NAMES)
+@pytest.mark.parametrize("leaf", [False, True])
+@pytest.mark.parametrize("main_grad", [False, True])
+def test_forward_mode_is_right_or_refused(device, which, leaf, main_grad):
+    """A tangent is never dropped: the CPU's operations carry it, the kernels refuse the call."""
+    import torch.autograd.forward_ad as fwd
+
+    c = _inputs(device, 5, 16, torch.float32)
+    t = {k: c[k].clone().requires_grad_(leaf) for k in NAMES}
+    with fwd.dual_level():
+        t[which] = fwd.make_dual(t[which], torch.ones_like(t[which]))
+        if main_grad:
+            t["pre_weight"].main_grad = torch.zeros(16, device=device)
+
+        def call():
+            y, s = ops.block_norm(t["h"], t["residual"], kind="layer", eps=EPS, **{k: t[k] for k in NAMES[2:]})
+            return fwd.unpack_dual(y).tangent
+
+        if device == "cpu":  # zero where a layer norm takes a constant away
+            got = call()
+            assert got is not None and (got.any() or which in ("h", "residual"))
+        else:
+            with pytest.raises(NotImplementedError):
+                call()
+            with torch.no_grad(), pytest.raises(NotImplementedError):
+                call()
+    if device == "cuda":
+        rest = {k: c[k] for k in NAMES if k != which}
+        with pytest.raises((NotImplementedError, RuntimeError)):
+            torch.func.jvp(lambda v: ops.block_norm(**rest, **{which: v}, eps=EPS), (c[which],), (torch.ones_like(c[which]),))

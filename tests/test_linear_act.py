@@ -413,3 +413,37 @@ def test_capture_beside_a_live_graph_is_refused(main_grad):
                                    (129, 184, 264), (65, 64, 56), (193, 128, 184), (257, 1016, 2040)])
 def test_last_step_of_a_single_row(device, m, k, n):
     _compare(_inputs(device, m, k, n, torch.bfloat16), "gelu")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("which", "xwbr")
+@pytest.mark.parametrize("leaf", [False, True])
+@pytest.mark.parametrize("main_grad", [False, True])
+def test_forward_mode_is_right_or_refused(device, which, leaf, main_grad):
+    """A tangent is never dropped: the CPU's operations carry it, the kernels refuse the call."""
+    import torch.autograd.forward_ad as fwd
+
+    c = _inputs(device, 5, 16, 8, torch.bfloat16)
+    t = {k: c[k].clone().requires_grad_(leaf) for k in "xwbr"}
+    if main_grad:
+        t["w"].main_grad = torch.zeros(8, 16, device=device)
+    with fwd.dual_level():
+        t[which] = fwd.make_dual(t[which], torch.ones_like(t[which]))
+        if main_grad and which == "w":
+            t["w"].main_grad = torch.zeros(8, 16, device=device)
+
+        def call():
+            return fwd.unpack_dual(ops.linear_act(t["x"], t["w"], t["b"], t["r"], "silu")).tangent
+
+        if device == "cpu":
+            got = call()
+            assert got is not None and got.any()
+        else:
+            with pytest.raises(NotImplementedError):
+                call()
+            with torch.no_grad(), pytest.raises(NotImplementedError):
+                call()
+    if device == "cuda":
+        with pytest.raises((NotImplementedError, RuntimeError)):
+            torch.func.jvp(lambda v: ops.linear_act(**{**{"x": c["x"], "weight": c["w"]}, {"x": "x", "w": "weight", "b": "bias", "r": "residual"}[which]: v}),
+                           (c[which],), (torch.ones_like(c[which]),))
