@@ -203,6 +203,24 @@ at::Tensor linear_act_dw(const at::Tensor& dz, const at::Tensor& x) {
   return dw;
 }
 
+// out [N, K] = dz^T x, or out + dz^T x: fp32, or dz's type.  Each element is read and written by one lane.
+void linear_act_dw_(const at::Tensor& out, const at::Tensor& dz, const at::Tensor& x, bool accumulate) {
+  TORCH_CHECK(dz.is_cuda() && dz.dim() == 2 && x.dim() == 2 && dz.size(0) == x.size(0) && dz.device() == x.device() &&
+                  dz.scalar_type() == x.scalar_type(),
+              "linear_act_dw_: dz ", dz.sizes(), ", x ", x.sizes());
+  TORCH_CHECK(out.device() == dz.device() && out.is_contiguous() && out.dim() == 2 && out.size(0) == dz.size(1) &&
+                  out.size(1) == x.size(1) && (out.scalar_type() == at::kFloat || out.scalar_type() == dz.scalar_type()),
+              "linear_act_dw_: out must be contiguous [", dz.size(1), ", ", x.size(1), "], fp32 or ", dz.scalar_type(),
+              ", got ", out.scalar_type(), " ", out.sizes());
+  c10::hip::HIPGuardMasqueradingAsCUDA g(dz.device());
+  auto zm = rows_of(dz), xm = rows_of(x);
+  st::LinearEpi e{};
+  e.out = out.data_ptr();
+  e.out_f32 = out.scalar_type() == at::kFloat;
+  if (accumulate) e.res = e.out;
+  product(zm, true, xm, true, e, dz.size(1), x.size(1), dz.size(0), aligned(out));
+}
+
 class LinearAct : public torch::autograd::Function<LinearAct> {
  public:
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w,
@@ -269,6 +287,7 @@ TORCH_LIBRARY_FRAGMENT(st_amd, m) {
   m.def("linear_act_dz(Tensor dy, Tensor? z, ScalarType type, int act, bool want_db, bool db_f32) -> (Tensor, Tensor)");
   m.def("linear_act_dx(Tensor dz, Tensor weight) -> Tensor");
   m.def("linear_act_dw(Tensor dz, Tensor x) -> Tensor");
+  m.def("linear_act_dw_(Tensor(a!) out, Tensor dz, Tensor x, bool accumulate) -> ()");
   m.def("check_capture(Tensor[] inputs) -> ()");
 }
 
@@ -278,6 +297,7 @@ TORCH_LIBRARY_IMPL(st_amd, CUDA, m) {
   m.impl("linear_act_dz", &linear_act_dz);
   m.impl("linear_act_dx", &linear_act_dx);
   m.impl("linear_act_dw", &linear_act_dw);
+  m.impl("linear_act_dw_", &linear_act_dw_);
   m.impl("check_capture", &check_capture);
 }
 

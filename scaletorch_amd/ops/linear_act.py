@@ -17,7 +17,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib
-from .grad import accumulate_grad, accumulate_linear_wgrad
+from .grad import _grad_ready, accumulate_grad, take_fresh
 
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
@@ -40,6 +40,17 @@ def linear_act_ref(x, weight, bias, residual, activation):
     if residual is None:
         return y.to(x.dtype)
     return (y + residual.to(f)).to(residual.dtype)
+
+
+def _weight_grad(weight, dz, x2):
+    """dz^T x2 into ``main_grad`` (None), or returned.  By linear_act's own product: the backward can be captured
+    into a graph, where a library product may not create its handle nor a tuner wait for its events."""
+    mg = getattr(weight, "main_grad", None)
+    if mg is None or not mg.is_contiguous() or mg.dtype not in (torch.float32, dz.dtype):
+        return accumulate_grad(weight, _lib.ops().linear_act_dw(dz, x2))
+    _lib.ops().linear_act_dw_(mg.view(weight.shape), dz, x2, not take_fresh(weight))
+    _grad_ready(weight)
+    return None
 
 
 class _LinearActFn(torch.autograd.Function):
@@ -66,8 +77,7 @@ class _LinearActFn(torch.autograd.Function):
             if nx:
                 dx = _lib.ops().linear_act_dx(dz, weight).view(x.shape)
             if nw:
-                dw = accumulate_linear_wgrad(weight, dz, x2) if getattr(weight, "main_grad", None) is not None \
-                    else _lib.ops().linear_act_dw(dz, x2)
+                dw = _weight_grad(weight, dz, x2)
             db = accumulate_grad(ctx.bias, db) if nb else None
         return dx, dw, db, dy if nr else None, None
 

@@ -447,3 +447,80 @@ def test_forward_mode_is_right_or_refused(device, which, leaf, main_grad):
         with pytest.raises((NotImplementedError, RuntimeError)):
             torch.func.jvp(lambda v: ops.linear_act(**{**{"x": c["x"], "weight": c["w"]}, {"x": "x", "w": "weight", "b": "bias", "r": "residual"}[which]: v}),
                            (c[which],), (torch.ones_like(c[which]),))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,k,n", [(1, 8, 4), (65, 65, 65), (777, 1024, 264), (328, 1544, 2056), (4100, 1024, 4096)])
+def test_main_grad_sums_in_fp32_and_in_its_own_type(m, k, n, dtype):
+    """dW added to an fp32 buffer, which is not rounded to 16 bits, and to a 16-bit one, rounded once; the first
+    gradient of a step overwrites."""
+    c = _inputs("cuda", m, k, n, dtype, False, False)
+    z = c["x"].double() @ c["w"].double().t()
+    dz = c["dy"].double() * (z > 0)
+    want, size = dz.t() @ c["x"].double(), dz.abs().t() @ c["x"].double().abs()
+    far = (z.abs() <= (k + 4) * U32 * (c["x"].double().abs() @ c["w"].double().abs().t())).double()
+    # relu keeps dz exact but where z is within its error of zero; then fp32 sums of m terms and the addition of 2
+    bound = (m + 4) * U32 * (size + 2) + (far * c["dy"].double().abs()).t() @ c["x"].double().abs()
+    for mt in (torch.float32, dtype):
+        w = c["w"].clone().requires_grad_(True)
+        w.main_grad = torch.full((n, k), 2.0, device="cuda", dtype=mt)
+        calls = []
+        w._st_grad_ready = calls.append
+        u = torch.finfo(mt).eps / 2
+        for fresh in (False, True):
+            w._st_fresh = fresh
+            old = 0.0 if fresh else 2.0
+            ops.linear_act(c["x"], w, activation="relu").backward(c["dy"])
+            assert ((w.main_grad.double() - old - want).abs() <= bound + 1.01 * u * (want + old).abs()).all()
+            assert not w._st_fresh
+        assert w.grad is None and calls == [w, w]
+
+
+@pytest.mark.gpu
+def test_main_grad_backward_needs_no_library(monkeypatch):
+    """Neither the library's products nor their tuner may run: both break a capture that meets them first."""
+    from scaletorch_amd.ops import grad
+
+    def refuse(*a, **k):
+        raise AssertionError("the weight gradient went to the tuned products")
+
+    monkeypatch.setattr(grad, "wgrad_into", refuse)
+    c = _inputs("cuda", 64, 64, 64, torch.bfloat16)
+    w = c["w"].clone().requires_grad_(True)
+    w.main_grad = torch.zeros(64, 64, device="cuda")
+    ops.linear_act(c["x"], w, c["b"], c["r"], "gelu").backward(c["dy"])
+    assert w.main_grad.any()
+
+
+@pytest.mark.gpu
+def test_main_grad_backward_is_captured():
+    """Forward and backward with main_grad in a graph without a pass before it, replayed between eager passes."""
+    c = _inputs("cuda", 200, 136, 264, torch.bfloat16)
+    t = {k: torch.nn.Parameter(c[k]) for k in "xwb"}
+    for k in "wb":
+        t[k].main_grad = torch.zeros(t[k].shape, device="cuda")
+
+    def step():
+        for k in "wb":
+            t[k].main_grad.zero_()
+        y = ops.linear_act(t["x"], t["w"], t["b"], activation="gelu")
+        (dx,) = torch.autograd.grad(y, [t["x"]], c["dy"])
+        return y.detach(), dx
+
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for seed in range(3):
+        new = _inputs("cuda", 200, 136, 264, torch.bfloat16, seed=seed + 5)
+        with torch.no_grad():
+            for k in "xwb":
+                t[k].copy_(new[k])
+        c["dy"].copy_(new["dy"])
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [v.clone() for v in (*outs, t["w"].main_grad, t["b"].main_grad)]
+        want = [*step(), t["w"].main_grad, t["b"].main_grad]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
