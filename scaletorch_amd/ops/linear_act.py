@@ -113,6 +113,7 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
         _check(x, weight, bias, residual)
         return linear_act_ref(x, weight, bias, residual, activation)
     if torch.is_autocast_enabled("cuda"):
+        _lib.check_capture(x, weight, bias, residual)  # a cast copy is no leaf: its accumulator would not be seen
         t = torch.get_autocast_dtype("cuda")
         x, weight, bias = (v if v is None else v.to(t) for v in (x, weight, bias))
     if getattr(weight, "main_grad", None) is not None or getattr(bias, "main_grad", None) is not None:

@@ -524,3 +524,24 @@ def test_main_grad_backward_is_captured():
         want = [*step(), t["w"].main_grad, t["b"].main_grad]
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("main_grad", [False, True])
+@pytest.mark.parametrize("held", ["linear", "cast"])
+def test_capture_beside_a_live_graph_is_refused_under_autocast(main_grad, held):
+    """The leaves are fp32 parameters whose 16-bit copies the operator takes.  Only the refusal is called: nothing of
+    it may be recorded."""
+    x, w, b = (torch.nn.Parameter(torch.randn(s, device="cuda")) for s in ((64, 64), (32, 64), (32,)))
+    if main_grad:
+        b.main_grad = torch.zeros(32, device="cuda")
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        live = ops.linear_act(x, w, b, activation="gelu") if held == "linear" else [v.bfloat16() for v in (x, w, b)]
+        torch.cuda.synchronize()
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            keep = torch.zeros(4, device="cuda")
+            with torch.no_grad():
+                y = ops.linear_act(x, w, b, activation="gelu")
+            with pytest.raises(RuntimeError, match="earlier autograd graph"):
+                ops.linear_act(x, w, b, activation="gelu")
+    del live, keep, y
