@@ -149,7 +149,7 @@ def block_norm(h: torch.Tensor, residual: torch.Tensor | None = None, *, kind: s
     # weights whose gradients live in an arena: the sums go there in fp32
     _check(h, residual, kind, post_weight, post_bias, gate, pre_weight, pre_bias)
     same = residual is None and post_weight is None and gate is None and scale == 1.0  # s is h itself
+    _lib.check_capture(h, residual, *weights)  # the caller's: a contiguous copy is no leaf
     hc, rc = h.contiguous(), None if residual is None else residual.contiguous()
-    _lib.check_capture(hc, rc, *weights)
     y, s = _BlockNormFn.apply(hc, rc, *weights, kind == "layer", float(scale), eps, not same)
     return y, h if same else s

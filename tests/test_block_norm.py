@@ -427,3 +427,21 @@ def test_forward_mode_is_right_or_refused(device, which, leaf, main_grad):
         rest = {k: c[k] for k in NAMES if k != which}
         with pytest.raises((NotImplementedError, RuntimeError)):
             torch.func.jvp(lambda v: ops.block_norm(**rest, **{which: v}, eps=EPS), (c[which],), (torch.ones_like(c[which]),))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("main_grad", [False, True])
+def test_capture_of_a_strided_leaf_beside_a_live_graph_is_refused(main_grad):
+    """The leaf itself is looked at, not the contiguous copy that the kernel reads."""
+    h = torch.nn.Parameter(torch.randn(64, 8, device="cuda").t())
+    w = torch.ones(64, device="cuda")
+    if main_grad:
+        w.main_grad = torch.zeros(64, device="cuda")
+    assert not h.is_contiguous()
+    live = h * 1
+    torch.cuda.synchronize()
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        keep = torch.zeros(4, device="cuda")
+        with pytest.raises(RuntimeError, match="earlier autograd graph"):
+            ops.block_norm(h, pre_weight=w)
+    del live, keep
