@@ -106,6 +106,11 @@ def _fusable(x: torch.Tensor) -> bool:
     return not x.is_cuda or x.dtype in (torch.bfloat16, torch.float16) or torch.is_autocast_enabled("cuda")
 
 
+def _drops(m: nn.Dropout) -> bool:
+    """Whether m changes its input: its own mode and rate, which a caller may have set apart from the model's."""
+    return m.training and m.p > 0
+
+
 class CausalSelfAttention(nn.Module):
     def __init__(self, cfg: GPTConfig):
         super().__init__()
@@ -127,9 +132,12 @@ class CausalSelfAttention(nn.Module):
         else:
             y = ops.flash_attn(q, k, v, causal=True)
         y = y.reshape(B, T, C)
-        if fused:
+        if fused:  # residual: only where self.out_dropout() leaves the output as it is
             return self.resid_dropout(ops.linear_act(y, self.c_proj.weight, self.c_proj.bias, residual))
         return self.resid_dropout(self.c_proj(y))
+
+    def out_dropout(self) -> nn.Dropout:
+        return self.resid_dropout
 
 
 class GELUMLP(nn.Module):
@@ -144,6 +152,9 @@ class GELUMLP(nn.Module):
             h = ops.linear_act(x, self.c_fc.weight, self.c_fc.bias, activation="gelu")
             return self.dropout(ops.linear_act(h, self.c_proj.weight, self.c_proj.bias, residual))
         return self.dropout(self.c_proj(F.gelu(self.c_fc(x))))
+
+    def out_dropout(self) -> nn.Dropout:
+        return self.dropout
 
 
 class Branch(nn.Module):
@@ -175,7 +186,7 @@ class Block(nn.Module):
         self.ln_1, self.attn = LayerNorm(cfg.n_embd, cfg.bias), CausalSelfAttention(cfg)
         self.ln_2, self.mlp = LayerNorm(cfg.n_embd, cfg.bias), GELUMLP(cfg)
         self.join_1, self.join_2 = Branch(cfg), Branch(cfg)
-        self.fused_ops, self.dropout = cfg.fused_ops, cfg.dropout
+        self.fused_ops = cfg.fused_ops
         if cfg.fused_ops:  # weights read without calling their modules: their buckets are waited for here
             self._st_reads = (self.ln_1, self.attn, self.ln_2, self.mlp, self.join_1, self.join_2)
 
@@ -187,16 +198,16 @@ class Block(nn.Module):
 
     def _fused(self, x):
         """The same through the fused operators.  A plain branch adds the residual in its projection's
-        epilogue (one stream less than adding it with the norm), unless dropout comes between."""
-        drop = self.dropout > 0 and self.training
+        epilogue (one stream less than adding it with the norm), unless dropout comes between: the dropout
+        module's own state tells, as in a model in eval mode whose dropout is left on."""
         y, _ = ops.block_norm(x, kind="layer", pre_weight=self.ln_1.weight, pre_bias=self.ln_1.bias, eps=1e-5)
-        y, x = self._join(self.attn, self.join_1, y, x, self.ln_2, drop)
-        return self._join(self.mlp, self.join_2, y, x, None, drop)[1]
+        y, x = self._join(self.attn, self.join_1, y, x, self.ln_2)
+        return self._join(self.mlp, self.join_2, y, x, None)[1]
 
     @staticmethod
-    def _join(block, branch, y, x, norm, drop):
+    def _join(block, branch, y, x, norm):
         w = {} if norm is None else dict(pre_weight=norm.weight, pre_bias=norm.bias)
-        if branch.plain and not drop:
+        if branch.plain and not _drops(block.out_dropout()):
             x = block(y, fused=True, residual=x)
             return ops.block_norm(x, kind="layer", eps=1e-5, **w)
         return ops.block_norm(block(y, fused=True), x, kind="layer", eps=1e-5, **branch.weights(), **w)

@@ -166,3 +166,22 @@ def test_generation_one_token_at_a_time():
     assert ((la - lb).norm() / la.norm()).item() <= 4 * 2.0 ** -8  # a few bf16 roundings apart
     out = b.generate(idx, 8, do_sample=False)
     assert out.shape == (1, 9) and (out < 97).all()
+
+
+@pytest.mark.parametrize("kw", VARIANTS)
+@pytest.mark.parametrize("mode", ["train", "eval with dropout on", "rate changed"])
+def test_dropout_comes_before_the_residual(kw, mode):
+    """fp32 on the CPU, the same random numbers: dropout falls on the branch's output, never on the residual stream,
+    whichever way it was switched on."""
+    out = {}
+    for fused in (False, True):
+        m = _model(fused, dropout=0.0 if mode == "rate changed" else 0.5, **kw)
+        m.train(mode == "train")
+        for d in m.modules():
+            if isinstance(d, torch.nn.Dropout):
+                d.train()
+                d.p = 0.5
+        torch.manual_seed(3)
+        out[fused] = m(torch.randint(0, 97, (2, 24), generator=torch.Generator().manual_seed(1)))[0]
+    # other orders of the same fp32 sums, as above
+    assert (out[True] - out[False]).norm() <= 1e-5 * out[False].norm()
