@@ -545,3 +545,32 @@ def test_capture_beside_a_live_graph_is_refused_under_autocast(main_grad, held):
             with pytest.raises(RuntimeError, match="earlier autograd graph"):
                 ops.linear_act(x, w, b, activation="gelu")
     del live, keep, y
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows", [3, 500])
+def test_tails_are_relative(device, act, dtype, rows):
+    """y and dx for z in [-9, 0], relative to the value itself, by an identity weight and an fp32 residual of zeros.
+
+    y = z s: s is a fit or sum of relative error 1e-6 at most times an exponential whose argument a (natural, up to
+    z^2 / 2 = 41, and 2 sqrt(2 / pi) (|z| + 0.045 |z|^3) = 67 in the tanh form) is off by 3 roundings of it, its
+    constants' included; in the tanh form, whose argument is a longer product, by up to 10."""
+    z = -(torch.arange(rows * 8) % 2305).float().div(256).to(dtype).view(rows, 8).to(device)
+    w = torch.eye(8, dtype=dtype, device=device)
+    x = z.clone().requires_grad_(True)
+    y = ops.linear_act(x, w, residual=torch.zeros(rows, 8, device=device), activation=act)
+    (dx,) = torch.autograd.grad(y, x, torch.ones_like(y))
+    r = z.double().requires_grad_(True)
+    from scaletorch_amd.ops.linear_act import _act_ref
+    ry = _act_ref(r, act)
+    (rdx,) = torch.autograd.grad(ry, r, torch.ones_like(ry))
+    a = {"gelu": r * r / 2, "gelu_tanh": 1.6 * (r.abs() + 0.045 * r.abs() ** 3), "silu": r.abs()}[act].detach()
+    rel = 1e-6 + ((10 if act == "gelu_tanh" else 3) * a + 16) * U32
+    assert ((y.double() - ry).abs() <= rel * ry.abs() + 1e-30).all()
+    # the slope is a sum of two such terms, s and z s'(z), of opposite signs; rounded to dx's type
+    size = torch.sigmoid(r).detach() if act == "silu" else torch.special.ndtr(r).detach()
+    size = size + (rdx - size).abs() if act != "gelu_tanh" else (ry / r.clamp_max(-1e-9)).detach().abs() + (rdx - (ry / r.clamp_max(-1e-9)).detach()).abs()
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 1e-30
+    assert ((dx.double() - rdx).abs() <= 2 * rel * size + 1.01 * torch.finfo(dtype).eps / 2 * rdx.abs() + tiny).all()
