@@ -103,7 +103,8 @@ class LayerNorm(nn.Module):
 
 def _fusable(x: torch.Tensor) -> bool:
     """Whether linear_act takes x: 16 bits (or made so by autocast) on the GPU, anything on the CPU."""
-    return not x.is_cuda or x.dtype in (torch.bfloat16, torch.float16) or torch.is_autocast_enabled("cuda")
+    return not x.is_cuda or x.dtype in (torch.bfloat16, torch.float16) or (
+        x.dtype == torch.float32 and torch.is_autocast_enabled("cuda"))
 
 
 def _drops(m: nn.Dropout) -> bool:

@@ -22,6 +22,11 @@ from .grad import _grad_ready, accumulate_grad, take_fresh
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
 
+def _autocast_type(x: torch.Tensor) -> torch.dtype | None:
+    kind = x.device.type
+    return torch.get_autocast_dtype(kind) if kind in ("cuda", "cpu") and torch.is_autocast_enabled(kind) else None
+
+
 def _act_ref(z: torch.Tensor, activation: str) -> torch.Tensor:
     if activation == "relu":
         return torch.relu(z)
@@ -35,6 +40,9 @@ def _act_ref(z: torch.Tensor, activation: str) -> torch.Tensor:
 def linear_act_ref(x, weight, bias, residual, activation):
     """The same from torch operations, in fp32 (float64 for float64 inputs)."""
     f = torch.float64 if x.dtype == torch.float64 else torch.float32
+    if _autocast_type(x) is not None:  # it would take F.linear back to 16 bits
+        with torch.autocast(x.device.type, enabled=False):
+            return linear_act_ref(x, weight, bias, residual, activation)
     z = F.linear(x.to(f), weight.to(f), None if bias is None else bias.to(f))
     y = _act_ref(z, activation)
     if residual is None:
@@ -104,18 +112,21 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     """``act(x weight^T + bias) + residual`` for x [..., K], weight [N, K], bias [N], residual [..., N].
 
     ``activation``: "none", "relu", "gelu", "gelu_tanh" or "silu".  On the GPU x, weight and bias are
-    bf16 or fp16 (under ``torch.autocast`` they are cast to its type); y has the residual's type,
-    which may be fp32, else x's.  Weight and bias gradients go to ``main_grad`` where it exists."""
+    bf16 or fp16; under ``torch.autocast`` they are cast as ``F.linear`` casts them, on the CPU too.  y has the
+    residual's type, which may be fp32, else x's.  Weight and bias gradients go to ``main_grad`` where it exists."""
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"linear_act: activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
-    if not _lib.use_native(x) or x.numel() == 0 or weight.numel() == 0:
+    t, native = _autocast_type(x), _lib.use_native(x)
+    if t is not None:
+        if native:
+            _lib.check_capture(x, weight, bias, residual)  # a cast copy is no leaf: its accumulator would not be seen
+        # what F.linear's cast leaves alone stays: fp64, whole numbers, other devices
+        x, weight, bias = (v.to(t) if v is not None and v.is_floating_point() and v.dtype != torch.float64
+                           and v.device.type == x.device.type else v for v in (x, weight, bias))
+    if not native or x.numel() == 0 or weight.numel() == 0:
         _check(x, weight, bias, residual)
         return linear_act_ref(x, weight, bias, residual, activation)
-    if torch.is_autocast_enabled("cuda"):
-        _lib.check_capture(x, weight, bias, residual)  # a cast copy is no leaf: its accumulator would not be seen
-        t = torch.get_autocast_dtype("cuda")
-        x, weight, bias = (v if v is None else v.to(t) for v in (x, weight, bias))
     if getattr(weight, "main_grad", None) is not None or getattr(bias, "main_grad", None) is not None:
         _lib.check_capture(x, weight, bias, residual)
         return _LinearActFn.apply(x, weight, bias, residual, act)

@@ -574,3 +574,35 @@ def test_tails_are_relative(device, act, dtype, rows):
     size = size + (rdx - size).abs() if act != "gelu_tanh" else (ry / r.clamp_max(-1e-9)).detach().abs() + (rdx - (ry / r.clamp_max(-1e-9)).detach()).abs()
     tiny = 2.0 ** -25 if dtype == torch.float16 else 1e-30
     assert ((dx.double() - rdx).abs() <= 2 * rel * size + 1.01 * torch.finfo(dtype).eps / 2 * rdx.abs() + tiny).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("rows", [0, 5])
+@pytest.mark.parametrize("xt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("residual", [None, torch.float32, torch.bfloat16])
+def test_autocast_casts_as_linear_does_everywhere(device, rows, xt, residual):
+    """On the CPU, without rows and with x already cast: F.linear's type, and the values of the cast operands."""
+    g = torch.Generator().manual_seed(0)
+    x, w, b = (torch.randn(s, generator=g).to(device) for s in ((rows, 64), (32, 64), (32,)))
+    x, r = x.to(xt), None if residual is None else torch.randn(rows, 32, generator=g).to(device, residual)
+    with torch.autocast(device, dtype=torch.bfloat16):
+        y, plain = ops.linear_act(x, w, b, r, "silu"), torch.nn.functional.linear(x, w, b)
+    assert y.dtype == (plain.dtype if r is None else r.dtype) and y.shape == plain.shape
+    assert torch.equal(y, ops.linear_act(x.bfloat16(), w.bfloat16(), b.bfloat16(), r, "silu"))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_autocast_leaves_other_types_alone(device):
+    """fp64 and whole numbers are not cast: refused on the GPU, fp64 products on the CPU."""
+    x, w = torch.randn(4, 16, device=device).double(), torch.randn(8, 16, device=device).double()
+    with torch.autocast(device, dtype=torch.bfloat16):
+        with pytest.raises(TypeError):
+            ops.linear_act(x.int(), w.int())
+        with pytest.raises(TypeError):
+            ops.linear_act(x, w.float())
+        if device == "cuda":
+            with pytest.raises(TypeError):
+                ops.linear_act(x, w)
+        else:
+            y = ops.linear_act(x, w)
+            assert y.dtype == torch.float64 and (y - x @ w.t()).abs().max() <= 1e-13
