@@ -56,28 +56,33 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(const P* __restrict__ dy
   st_lane<VEC>(partial + (int64_t)blockIdx.y * width + c0, lane, 64, left, acc);
 }
 
-// db from the runs' sums: 32 columns a workgroup, 32 groups of runs
+// db from the runs' sums: 32 columns a workgroup at a time, 32 groups of runs
 template <typename T>
 __global__ __launch_bounds__(1024) void linear_db_kernel(const float* __restrict__ partial, int runs, int width,
                                                          T* __restrict__ db, float* __restrict__ db32) {
   __shared__ float red[32][33];
-  const int q = threadIdx.x & 31, g = threadIdx.x >> 5, col = blockIdx.x * 32 + q;
-  float s[4] = {0.f, 0.f, 0.f, 0.f};
-  if (col < width) {
-    int b = g;
-    for (; b + 96 < runs; b += 128)
+  const int q = threadIdx.x & 31, g = threadIdx.x >> 5;
+  for (int64_t c0 = (int64_t)blockIdx.x * 32; c0 < width; c0 += (int64_t)gridDim.x * 32) {
+    const int64_t col = c0 + q;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    if (col < width) {
+      int b = g;
+      for (; b + 96 < runs; b += 128)
 #pragma unroll
-      for (int u = 0; u < 4; ++u) s[u] += partial[(int64_t)(b + 32 * u) * width + col];
-    for (; b < runs; b += 32) s[0] += partial[(int64_t)b * width + col];
+        for (int u = 0; u < 4; ++u) s[u] += partial[(int64_t)(b + 32 * u) * width + col];
+      for (; b < runs; b += 32) s[0] += partial[(int64_t)b * width + col];
+    }
+    red[g][q] = (s[0] + s[1]) + (s[2] + s[3]);
+    __syncthreads();
+    if (!g && col < width) {
+      float t = red[0][q];
+      for (int i = 1; i < 32; ++i) t += red[i][q];
+      const float f[1] = {t};
+      if (db32) st_row<1>(db32 + col, f);
+      else st_row<1>(db + col, f);
+    }
+    __syncthreads();
   }
-  red[g][q] = (s[0] + s[1]) + (s[2] + s[3]);
-  __syncthreads();
-  if (g || col >= width) return;
-  float t = red[0][q];
-  for (int i = 1; i < 32; ++i) t += red[i][q];
-  const float f[1] = {t};
-  if (db32) st_row<1>(db32 + col, f);
-  else st_row<1>(db + col, f);
 }
 
 template <typename P, typename T>
@@ -90,9 +95,11 @@ int launch(const void* dy, const void* z, void* dz, void* db, int db_f32, float*
     linear_dz_kernel<P, T, 8><<<grid, 256, 0, st>>>((const P*)dy, (const T*)z, (T*)dz, part, rows, width, run, act);
   else
     linear_dz_kernel<P, T, 1><<<grid, 256, 0, st>>>((const P*)dy, (const T*)z, (T*)dz, part, rows, width, run, act);
-  if (db)
-    linear_db_kernel<T><<<(unsigned)((width + 31) / 32), 1024, 0, st>>>(part, runs, width, db_f32 ? nullptr : (T*)db,
-                                                                        db_f32 ? (float*)db : nullptr);
+  if (db) {
+    const unsigned blocks = (unsigned)std::min((width + 31) / 32, 1 << 21);  // a grid holds fewer than 2^32 threads
+    linear_db_kernel<T><<<blocks, 1024, 0, st>>>(part, runs, width, db_f32 ? nullptr : (T*)db,
+                                                 db_f32 ? (float*)db : nullptr);
+  }
   return (int)hipGetLastError();
 }
 

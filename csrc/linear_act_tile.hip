@@ -143,7 +143,9 @@ __global__ __launch_bounds__(NT) void linear_tile_kernel(LinearArgs p) {
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wid >> 1, wn = wid & 1;
   const int nbn = (p.N + BN - 1) / BN, nbm = (p.M + BM - 1) / BM;
-  const int vb = xcd_remap((int)blockIdx.x, nbm * nbn);
+  const uint32_t wg = blockIdx.z * gridDim.x + blockIdx.x;  // launch: the tiles over x and z
+  if (wg >= (uint32_t)(nbm * nbn)) return;
+  const int vb = xcd_remap((int)wg, nbm * nbn);
   // groups of 8 row blocks: the tiles an XCD holds at once share operand slices in its L2
   const int per = 8 * nbn, grp = vb / per, in = vb % per, gsz = min(8, nbm - grp * 8);
   const int m0 = (grp * 8 + in % gsz) * BM, n0 = (in / gsz) * BN;
@@ -276,7 +278,8 @@ template <int BM, int BN, bool ACOL, bool BCOL, int AHEAD = BM + BN < 256 ? 4 : 
 int launch(const LinearArgs& p, hipStream_t st) {
   const int64_t tiles = (int64_t)((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
   if (tiles >= (1LL << 31)) return -2;
-  const dim3 grid((unsigned)tiles, (unsigned)p.splits);
+  const int64_t most = 1 << 23;  // a dimension of a grid holds fewer than 2^32 threads
+  const dim3 grid((unsigned)std::min(tiles, most), (unsigned)p.splits, (unsigned)((tiles + most - 1) / most));
   if (p.vec) {
     if (p.epi.f16) linear_tile_kernel<BM, BN, AHEAD, ACOL, BCOL, true, true><<<grid, NT, 0, st>>>(p);
     else linear_tile_kernel<BM, BN, AHEAD, ACOL, BCOL, true, false><<<grid, NT, 0, st>>>(p);

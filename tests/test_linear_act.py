@@ -606,3 +606,38 @@ def test_autocast_leaves_other_types_alone(device):
         else:
             y = ops.linear_act(x, w)
             assert y.dtype == torch.float64 and (y - x @ w.t()).abs().max() <= 1e-13
+
+
+@pytest.mark.gpu
+def test_more_tiles_than_a_grid_dimension_holds():
+    """2^24 + 2 tiles of 64 rows, and the backward; every value is exact."""
+    m = (1 << 30) + 70
+    if torch.cuda.mem_get_info()[0] < 30e9:
+        pytest.skip("needs 30 GB")
+    x = torch.randn(m, 1, device="cuda", dtype=torch.bfloat16, generator=torch.Generator("cuda").manual_seed(0)).requires_grad_(True)
+    w = torch.ones(1, 1, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    y = ops.linear_act(x, w, activation="relu")
+    assert torch.equal(y, x.detach().clamp_min(0))
+    dy = torch.zeros_like(y)
+    ends = [0, 1, 1 << 29, m - 71, m - 2, m - 1]
+    dy[ends] = 2.0
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    pos = (x.detach()[ends] > 0).to(dx.dtype)
+    assert torch.equal(dx[ends], 2 * pos) and dx.count_nonzero() == pos.count_nonzero()
+    want = (2 * pos.double() * x.detach()[ends].double()).sum()
+    assert abs(dw.double().item() - want.item()) <= (2.0 ** -8 + 8 * U32) * want.abs().item() + 1e-6
+
+
+@pytest.mark.gpu
+def test_more_columns_than_a_grid_dimension_holds():
+    """The bias gradient of 2^27 + 40 columns."""
+    n = (1 << 27) + 40
+    if torch.cuda.mem_get_info()[0] < 10e9:
+        pytest.skip("needs 10 GB")
+    x = torch.ones(1, 1, device="cuda", dtype=torch.bfloat16)
+    w = torch.ones(n, 1, device="cuda", dtype=torch.bfloat16)
+    b = torch.zeros(n, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    y = ops.linear_act(x, w, b, activation="relu")
+    dy = torch.randn(1, n, device="cuda", dtype=torch.bfloat16, generator=torch.Generator("cuda").manual_seed(0))
+    (db,) = torch.autograd.grad(y, b, dy)
+    assert (y == 1).all() and torch.equal(db, dy[0])
