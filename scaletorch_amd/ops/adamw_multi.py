@@ -199,8 +199,11 @@ def adamw_multi_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], 
                                "run the step outside the graph")
         _lib.ops().adamw_multi_.default(params, grads, exp_avg, exp_avg_sq, _some(masters), _some(scales), clip_coef,
                                         wd, lr, b1, b2, eps, step, scale_grads)
-        # the kernel writes behind autograd's back: a graph that saved a parameter has to notice
-        torch.autograd.graph.increment_version([*params, *grads] if scale_grads else params)
+        # the kernel writes behind autograd's back: a graph that saved what it wrote has to notice
+        written = [*params, *exp_avg, *exp_avg_sq, *(masters or ()), *(scales or ())]
+        if scale_grads and clip_coef is not None:
+            written += grads
+        torch.autograd.graph.increment_version([t for t in written if t is not None])
         return
     masters = [None] * n if masters is None else masters
     scales = [None] * n if scales is None else scales

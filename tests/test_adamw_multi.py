@@ -447,3 +447,17 @@ def test_forward_mode_is_refused(which):
         with pytest.raises(NotImplementedError):
             ops.adamw_multi_(**d, step=1, lr=1e-3, clip_coef=clip)
     assert all(torch.equal(a, b) for k in ("params", "exp_avg", "exp_avg_sq") for a, b in zip(c[k], before[k]))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("which", ["params", "masters", "exp_avg", "exp_avg_sq", "scales", "grads"])
+def test_a_graph_that_saved_what_a_step_writes_notices(device, which):
+    """On the GPU as on the CPU: backward through an overwritten value raises."""
+    eight = which == "scales"
+    c = _case([(300,)], device, torch.bfloat16, torch.float32, eight)
+    one = torch.ones((), device=device, requires_grad=True)
+    y = (one * c[which][0]).sum()  # saves the second factor
+    kw = dict(clip_coef=torch.full((1,), 0.5, device=device), scale_grads=True) if which == "grads" else {}
+    ops.adamw_multi_(**c, step=1, lr=1e-3, **kw)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
