@@ -50,6 +50,10 @@ def block_norm_ref(h, residual, layer, post_weight, post_bias, gate, scale, pre_
     return y, s.to(h.dtype if residual is None else residual.dtype)
 
 
+def _flat(*weights):
+    return [None if w is None else w.contiguous() for w in weights]
+
+
 class _BlockNormFn(torch.autograd.Function):
     """For weights with ``main_grad``; without, csrc/block_norm_ops.cpp has the same in C++."""
 
@@ -57,7 +61,8 @@ class _BlockNormFn(torch.autograd.Function):
     def forward(ctx, h, residual, gate, w1, b1, w2, b2, layer, scale, eps, write_s):
         stream = h.dtype if residual is None else residual.dtype
         alone = w1 is None and gate is None and (not write_s or stream == torch.float32)
-        y, s, stats = _lib.ops().block_norm_fwd(h, residual, gate, w1, b1, w2, b2, layer, scale, eps, write_s, True)
+        y, s, stats = _lib.ops().block_norm_fwd(h, residual, *_flat(gate, w1, b1, w2, b2), layer, scale, eps, write_s,
+                                                True)
         y = y if w2 is not None else None
         s = s if write_s else None
         # what the backward recomputes from (csrc/block_norm_bwd.hip): h and the residual, or s alone
@@ -84,7 +89,7 @@ class _BlockNormFn(torch.autograd.Function):
         weights = (gate, w1, b1, w2, b2)
         f32 = [0, 0] + [int(w is not None and getattr(w, "main_grad", None) is not None) for w in weights]
         got = _lib.ops().block_norm_bwd(None if dy is None else dy.contiguous(), None if ds is None else ds.contiguous(),
-                                        h, residual, s, stats, gate, w1, b1, w2, b2, layer, scale, eps,
+                                        h, residual, s, stats, *_flat(*weights), layer, scale, eps,
                                         [int(w) for w in want], f32, htype)
         got = [g if w else None for g, w in zip(got, want)]
         if one and need[0]:

@@ -445,3 +445,25 @@ def test_capture_of_a_strided_leaf_beside_a_live_graph_is_refused(main_grad):
         with pytest.raises(RuntimeError, match="earlier autograd graph"):
             ops.block_norm(h, pre_weight=w)
     del live, keep
+
+
+@pytest.mark.gpu
+def test_strided_and_expanded_weights_beside_main_grad():
+    """A gate that is one value expanded, a bias that is a column of something wider."""
+    c = _inputs("cuda", 40, 264, torch.bfloat16)
+
+    def run(main_grad):
+        g = c["gate"][:1].clone().requires_grad_(True)
+        wide = torch.stack([c["pre_bias"], c["post_bias"]], 1).requires_grad_(True)
+        w = c["pre_weight"].clone().requires_grad_(True)
+        if main_grad:
+            w.main_grad = torch.zeros(264, device="cuda")
+        y, s = ops.block_norm(c["h"], c["residual"], kind="layer", post_weight=c["post_weight"], post_bias=wide[:, 1],
+                              gate=g.expand(264), pre_weight=w, pre_bias=wide[:, 0], eps=EPS)
+        torch.autograd.backward((y, s), (c["dy"], c["ds"]))
+        return y, s, g.grad, wide.grad, (w.main_grad if main_grad else w.grad)
+
+    for a, b in zip(run(True)[:4], run(False)):
+        assert torch.equal(a, b)
+    w32, w16 = run(True)[4], run(False)[4]
+    assert torch.equal(w32.bfloat16(), w16)  # the same sums, rounded once
