@@ -461,3 +461,60 @@ def test_a_graph_that_saved_what_a_step_writes_notices(device, which):
     ops.adamw_multi_(**c, step=1, lr=1e-3, **kw)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ptype,gtype", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.float16, torch.float32)])
+@pytest.mark.parametrize("shifted", [("params", "grads", "masters"), ("grads",), ("exp_avg", "exp_avg_sq"), ("exp_avg_sq",),
+                                     ("params", "grads", "masters", "exp_avg", "exp_avg_sq")])
+def test_eight_bits_with_shifted_tensors(ptype, gtype, shifted):
+    """Element by element where a tensor is not aligned for four at once: the same operations, the same bits."""
+    a = _case(SIZES, "cuda", ptype, gtype, True, seed=7)
+    b = _clone(a)
+    for k in shifted:
+        for i, t in enumerate(b[k]):
+            if t is not None:
+                b[k][i] = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")[1:].copy_(t.reshape(-1)).view(t.shape)
+    for step in (1, 2):
+        for c in (a, b):
+            ops.adamw_multi_(**c, step=step, weight_decay=0.1, **HYPER)
+    for k in a:
+        for x, y in zip(a[k], b[k]):
+            assert x is None or torch.equal(x.view(torch.uint8) if x.dtype == F8 else x, y.view(torch.uint8) if y.dtype == F8 else y)
+
+
+@pytest.mark.gpu
+def test_places_past_32_bits_enter_the_hash():
+    """The codes of a tensor behind 2^32 elements of the call: rounding offsets of its place, both words of it.
+    beta1 = 0, so the first moment is the gradient."""
+    big, n, step = 1 << 32, 4000, 9
+    if torch.cuda.mem_get_info()[0] < 40e9:
+        pytest.skip("needs 40 GB")
+    z = lambda m, dt=torch.float32: torch.zeros(m, dtype=dt, device="cuda")  # noqa: E731
+    g = torch.randn(n, generator=torch.Generator().manual_seed(0))
+    c = dict(params=[z(big), z(n)], grads=[z(big, torch.bfloat16), g.cuda()], exp_avg=[z(big, F8), z(n, F8)],
+             exp_avg_sq=[z(big, F8), z(n, F8)], scales=[z(2 * ops.adamw_blocks(big)).view(-1, 2), z(2 * ops.adamw_blocks(n)).view(-1, 2)])
+    ops.adamw_multi_(**c, step=step, lr=1e-3, betas=(0.0, 0.0))
+    got = c["exp_avg"][1].cpu()
+
+    def mix(x):
+        x ^= x >> 16
+        x = x * 0x7FEB352D & 0xFFFFFFFF
+        x ^= x >> 15
+        x = x * 0x846CA68B & 0xFFFFFFFF
+        return x ^ x >> 16
+
+    def codes(place):
+        key = mix(step * 0x9E3779B9 & 0xFFFFFFFF)
+        r16 = [mix((i & 0xFFFFFFFF) ^ mix(i >> 32 ^ key)) & 0xFFFF for i in range(place, place + n)]
+        top = torch.nn.functional.pad(g, (0, -n % 256)).view(-1, 256).abs().amax(1).double().repeat_interleave(256)[:n]
+        a = g.double().abs() * 448 / top
+        unit = torch.exp2(torch.floor(torch.log2(a.clamp_min(2.0 ** -6))) - 3)  # e4m3's step there
+        q = ((a / unit + torch.tensor(r16).double() / 65536).floor() * unit).clamp_max(448)
+        return (q * g.sign()).float().to(F8)
+
+    off = _code_steps(got, codes(big))
+    # next to a border the fp32 scaling may fall on its other side: 2^-23 of a value over a step of 2^-3 of it
+    assert off.max() <= 1 and (off > 0).sum() <= 2
+    assert (_code_steps(got, codes(0)) > 0).float().mean() > 0.1  # another place, other offsets
+    assert not c["exp_avg"][0].view(torch.uint8).any()
