@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import inspect
 import math
+import warnings
 from dataclasses import dataclass, field
 
 import torch
@@ -192,8 +193,11 @@ class Block(nn.Module):
             self._st_reads = (self.ln_1, self.attn, self.ln_2, self.mlp, self.join_1, self.join_2)
 
     def forward(self, x):
-        if self.fused_ops and _fusable(x):
-            return self._fused(x)
+        if self.fused_ops:
+            if _fusable(x):
+                return self._fused(x)
+            warnings.warn(f"GPT fused_ops: blocks of {x.dtype} activations on the GPU run unfused (the fused operators "
+                          "take 16 bits, or fp32 under torch.autocast)", stacklevel=2)
         x = self.join_1(x, self.attn(self.ln_1(x)))
         return self.join_2(x, self.mlp(self.ln_2(x)))
 

@@ -185,3 +185,18 @@ def test_dropout_comes_before_the_residual(kw, mode):
         out[fused] = m(torch.randint(0, 97, (2, 24), generator=torch.Generator().manual_seed(1)))[0]
     # other orders of the same fp32 sums, as above
     assert (out[True] - out[False]).norm() <= 1e-5 * out[False].norm()
+
+
+@pytest.mark.gpu
+def test_an_fp32_model_on_the_gpu_says_that_it_runs_unfused():
+    import warnings
+
+    idx = torch.randint(0, 97, (2, 32), device="cuda")
+    with torch.no_grad():
+        want = _model(False).cuda()(idx)[0]
+        with pytest.warns(UserWarning, match="unfused"):
+            got = _model(True).cuda()(idx)[0]
+        assert torch.equal(got, want)
+        with warnings.catch_warnings():
+            warnings.simplefilter("error")
+            _model(True).cuda().bfloat16()(idx)
