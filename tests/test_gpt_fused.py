@@ -200,3 +200,23 @@ def test_an_fp32_model_on_the_gpu_says_that_it_runs_unfused():
         with warnings.catch_warnings():
             warnings.simplefilter("error")
             _model(True).cuda().bfloat16()(idx)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", VARIANTS)
+def test_arenas_under_autocast(kw):
+    """fp32 parameters in arenas, 16-bit products: the gradients of the bare model, over two accumulated passes."""
+    from scaletorch_amd.parallel.data_parallel import DataParallel
+
+    idx = torch.randint(0, 97, (2, 64), device="cuda")
+    bare, inner = (_model(True, **kw).cuda() for _ in range(2))
+    _, want = _grads(bare, idx, torch.bfloat16)
+    dp = DataParallel(inner, bucket_size=1 << 16, expose_grads=True)
+    for _ in range(2):
+        dp.zero_grad()
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            loss = dp(idx, idx)[1]
+        loss.backward()
+        got = {n: p.grad.double() for n, p in inner.named_parameters()}
+        # the same products; only fp32 sums of the norms' weights may be added up in another order
+        assert max(_off(got, want).values()) <= 1e-5
