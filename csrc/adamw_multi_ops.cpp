@@ -10,6 +10,7 @@
 #include <vector>
 
 #include "adamw_multi.h"
+#include "capture_check.h"
 #include "forward_grad_check.h"
 
 extern "C" int st_adamw_multi(const AdamTable* tab, int count, const AdamScalars* h, int gtype, int ptype, int eight,
@@ -53,6 +54,11 @@ void adamw_multi_(at::TensorList params, at::TensorList grads, at::TensorList ex
   for (const at::TensorList l : {params, grads, exp_avg, exp_avg_sq, masters, scales})
     st::refuse_forward_grad(l, "adamw_multi");
   const auto dev = params[0].device();
+  TORCH_CHECK(dev.is_cuda(), "adamw_multi: param 0 must be on a GPU, got ", dev);
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+  const auto current = c10::hip::getCurrentHIPStream();
+  TORCH_CHECK(!st::is_capturing(current), "adamw_multi: the step number is the host's, so a captured step would repeat "
+              "it; run the step outside the graph");
   auto check = [&](const at::Tensor& t, int64_t n, const char* what, size_t i) {
     TORCH_CHECK(t.is_cuda() && t.device() == dev, "adamw_multi: ", what, " ", i, " must be on ", dev, ", got ",
                 t.device());
@@ -143,8 +149,7 @@ void adamw_multi_(at::TensorList params, at::TensorList grads, at::TensorList ex
                 "adamw_multi: two of the tensors share memory (or one is given twice)");
     (s.written ? end_written : end_read) = std::max(s.written ? end_written : end_read, s.hi);
   }
-  c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
-  const hipStream_t stream = c10::hip::getCurrentHIPStream().stream();
+  const hipStream_t stream = current.stream();
   AdamTable tab;
   for (int k = 0; k < 18; ++k) {
     int count = 0;

@@ -72,7 +72,10 @@ def ops():
 def check_capture(*inputs: torch.Tensor | None) -> None:
     """Refuses a training call under graph capture whose gradients would be accumulated on another
     stream, that of an earlier autograd graph still held (csrc/capture_check.h)."""
-    if torch.is_grad_enabled() and torch.cuda.is_current_stream_capturing():
+    if not torch.is_grad_enabled():
+        return
+    here = all(t is None or t.device.index == torch.cuda.current_device() for t in inputs)
+    if not here or torch.cuda.is_current_stream_capturing():
         ops().check_capture([t for t in inputs if t is not None])
 
 

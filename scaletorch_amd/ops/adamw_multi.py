@@ -194,9 +194,6 @@ def adamw_multi_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], 
     if not n:
         return
     if _lib.use_native(params[0]):
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("adamw_multi: the step number is the host's, so a captured step would repeat it; "
-                               "run the step outside the graph")
         _lib.ops().adamw_multi_.default(params, grads, exp_avg, exp_avg_sq, _some(masters), _some(scales), clip_coef,
                                         wd, lr, b1, b2, eps, step, scale_grads)
         # the kernel writes behind autograd's back: a graph that saved what it wrote has to notice
