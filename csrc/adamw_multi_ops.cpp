@@ -51,8 +51,7 @@ void adamw_multi_(at::TensorList params, at::TensorList grads, at::TensorList ex
               "adamw_multi: lists of different lengths");
   if (N == 0) return;
   TORCH_CHECK(step >= 1 && step <= UINT32_MAX, "adamw_multi: step counts from 1, got ", step);
-  for (const at::TensorList l : {params, grads, exp_avg, exp_avg_sq, masters, scales})
-    st::refuse_forward_grad(l, "adamw_multi");
+  st::refuse_forward_grad({params, grads, exp_avg, exp_avg_sq, masters, scales}, "adamw_multi");
   const auto dev = params[0].device();
   TORCH_CHECK(dev.is_cuda(), "adamw_multi: param 0 must be on a GPU, got ", dev);
   c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
@@ -67,7 +66,7 @@ void adamw_multi_(at::TensorList params, at::TensorList grads, at::TensorList ex
   };
   AdamScalars h{};
   if (clip_coef.has_value() && clip_coef->defined()) {
-    st::refuse_forward_grad(*clip_coef, "adamw_multi");
+    st::refuse_forward_grad({&*clip_coef}, "adamw_multi");
     check(*clip_coef, 1, "clip_coef", 0);
     TORCH_CHECK(clip_coef->scalar_type() == at::kFloat, "adamw_multi: clip_coef must be fp32");
     h.clip = clip_coef->data_ptr<float>();
@@ -172,6 +171,12 @@ void adamw_multi_(at::TensorList params, at::TensorList grads, at::TensorList ex
     }
     flush();
   }
+  // the kernel writes behind autograd's back: a graph that saved what it wrote has to notice
+  for (const at::TensorList l : {params, exp_avg, exp_avg_sq, masters, scales})
+    for (const auto& t : l)
+      if (t.defined()) t.unsafeGetTensorImpl()->bump_version();
+  if (h.write_grads)
+    for (const auto& t : grads) t.unsafeGetTensorImpl()->bump_version();
 }
 
 }  // namespace

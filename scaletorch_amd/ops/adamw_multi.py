@@ -196,11 +196,6 @@ def adamw_multi_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], 
     if _lib.use_native(params[0]):
         _lib.ops().adamw_multi_.default(params, grads, exp_avg, exp_avg_sq, _some(masters), _some(scales), clip_coef,
                                         wd, lr, b1, b2, eps, step, scale_grads)
-        # the kernel writes behind autograd's back: a graph that saved what it wrote has to notice
-        written = [*params, *exp_avg, *exp_avg_sq, *(masters or ()), *(scales or ())]
-        if scale_grads and clip_coef is not None:
-            written += grads
-        torch.autograd.graph.increment_version([t for t in written if t is not None])
         return
     masters = [None] * n if masters is None else masters
     scales = [None] * n if scales is None else scales
