@@ -22,7 +22,7 @@ struct NormArgs {
   // backward
   const void *dy, *ds;  // null: zero
   void *dh, *dres;      // null: not wanted
-  float* partial;       // [blocks, arrays, width] column sums
+  float* partial;       // column sums [blocks, arrays, width]; from the host: the workspace that holds them
   int64_t rows;
   int width;
   int layer;            // 0 RMS, 1 layer norm

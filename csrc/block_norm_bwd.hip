@@ -146,15 +146,17 @@ __global__ __launch_bounds__(MOST) void block_norm_bwd_kernel(NormArgs a) {
 }
 
 // The workgroups' partial sums [blocks][arrays][width] in kParts parts of blocks each: a wave 64
-// columns, four waves a quarter of the part each, added in order.
+// columns, four waves a quarter of the part each, added in order.  From here on sums are held in 64
+// bits: a scalar gate's gradient is one sum over all columns, in which the columns' sums cancel (in fp32
+// that of 3001 x 1001 was off by up to 1e-6 of itself, as much as five times the rows' own sums are).
 constexpr int kParts = 8;
 __global__ __launch_bounds__(256) void block_norm_colsum_kernel(const float* __restrict__ partial, int blocks,
-                                                                int arrays, int width, float* __restrict__ out) {
-  __shared__ float red[4][64];
+                                                                int arrays, int width, double* __restrict__ out) {
+  __shared__ double red[4][64];
   const int q = threadIdx.x & 63, g = threadIdx.x >> 6, col = blockIdx.x * 64 + q;
   const int64_t line = (int64_t)arrays * width, at = (int64_t)blockIdx.y * width + col;
   const int per = (blocks + kParts - 1) / kParts, b1 = min(blocks, (int)(blockIdx.z + 1) * per);
-  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  double s[4] = {0., 0., 0., 0.};
   if (col < width) {
     int b = blockIdx.z * per + g;
     for (; b + 12 < b1; b += 16)
@@ -167,8 +169,10 @@ __global__ __launch_bounds__(256) void block_norm_colsum_kernel(const float* __r
   if (!g && col < width) out[blockIdx.z * line + at] = (red[0][q] + red[1][q]) + (red[2][q] + red[3][q]);
 }
 
+int64_t sum_floats(int arrays, int width) { return (int64_t)kParts * arrays * width * 2; }  // whole 64 bytes
+
 struct FinishArgs {
-  const float* sums;  // [kParts][arrays][width]
+  const double* sums;  // [kParts][arrays][width]
   int arrays, width;
   int gen;
   const void *gate, *w1, *b1;
@@ -188,35 +192,36 @@ ST_DEVICE void put(void* p, int f32, int i, float v) {
 // One column a thread; with a scalar gate one workgroup takes all columns and adds up their gates.
 template <typename T>
 __global__ __launch_bounds__(1024) void block_norm_finish_kernel(FinishArgs f) {
-  __shared__ float red[16];
-  float total = 0.f;
+  __shared__ double red[16];
+  double total = 0.;
   for (int col = blockIdx.x * blockDim.x + threadIdx.x; col < f.width; col += gridDim.x * blockDim.x) {
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    double s[4] = {0., 0., 0., 0.};
 #pragma unroll
     for (int b = 0; b < kParts; ++b)
 #pragma unroll
       for (int k = 0; k < 4; ++k)
         s[k] += f.sums[((int64_t)b * f.arrays + (k < f.arrays ? k : 0)) * f.width + col];  // no branch: all in flight
-    const float A = s[1], dyb = s[f.gen ? 2 : 1], B = s[3];
-    if (f.dw2) put<T>(f.dw2, f.tw2, col, s[0]);
-    if (f.db2) put<T>(f.db2, f.tb2, col, dyb);
+    const double A = s[1], dyb = s[f.gen ? 2 : 1], B = s[3];
+    if (f.dw2) put<T>(f.dw2, f.tw2, col, (float)s[0]);
+    if (f.db2) put<T>(f.db2, f.tb2, col, (float)dyb);
     if (f.gen) {
-      const float w = f.w1 ? ld_one<T>(f.w1, f.w32, col) : 1.f, b = f.b1 ? ld_one<T>(f.b1, f.w32, col) : 0.f;
-      const float k = f.scale * (f.gate_n ? ld_one<T>(f.gate, f.w32, f.gate_n > 1 ? col : 0) : 1.f);
-      if (f.dw1) put<T>(f.dw1, f.tw1, col, k * A);
-      if (f.db1) put<T>(f.db1, f.tb1, col, k * B);
-      const float dg = f.scale * (w * A + (f.b1 ? b * B : 0.f));
-      if (f.dgate && f.gate_n > 1) put<T>(f.dgate, f.tgate, col, dg);
+      const double w = f.w1 ? ld_one<T>(f.w1, f.w32, col) : 1.f, b = f.b1 ? ld_one<T>(f.b1, f.w32, col) : 0.f;
+      const double k = (double)f.scale * (f.gate_n ? ld_one<T>(f.gate, f.w32, f.gate_n > 1 ? col : 0) : 1.f);
+      if (f.dw1) put<T>(f.dw1, f.tw1, col, (float)(k * A));
+      if (f.db1) put<T>(f.db1, f.tb1, col, (float)(k * B));
+      const double dg = f.scale * (w * A + (f.b1 ? b * B : 0.));
+      if (f.dgate && f.gate_n > 1) put<T>(f.dgate, f.tgate, col, (float)dg);
       total += dg;
     }
   }
   if (f.gate_n != 1 || !f.dgate) return;
-  total = wave_sum(total);
+#pragma unroll
+  for (int off = 32; off; off >>= 1) total += __shfl_xor(total, off);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = total;
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int i = 1; i < 16; ++i) total += red[i];
-    put<T>(f.dgate, f.tgate, 0, total);
+    put<T>(f.dgate, f.tgate, 0, (float)total);
   }
 }
 
@@ -263,9 +268,13 @@ int st_block_norm_bwd_blocks(int64_t rows, int width) {
   return (int)(need < most ? need : most);
 }
 
-int st_block_norm_bwd(const NormArgs* a, int gen, int bias, int blocks, int htype, int stype, int vec, hipStream_t st) {
-  if (a->rows <= 0 || a->width <= 0 || a->width > kNormMaxWidth || (vec && a->width % 8) || blocks <= 0) return -2;
-  if (!gen && !a->s && (stype == kF32 || !a->h)) return -2;
+int st_block_norm_bwd(const NormArgs* args, int gen, int bias, int blocks, int htype, int stype, int vec, hipStream_t st) {
+  if (args->rows <= 0 || args->width <= 0 || args->width > kNormMaxWidth || (vec && args->width % 8) || blocks <= 0)
+    return -2;
+  if (!gen && !args->s && (stype == kF32 || !args->h)) return -2;
+  NormArgs shifted = *args;
+  if (shifted.partial) shifted.partial += sum_floats((gen ? 2 : 1) * (bias ? 2 : 1), args->width);
+  const NormArgs* a = &shifted;
   if (htype == kF32 && stype == kF32) return launch<float, float>(*a, gen, bias, blocks, vec, st);
   if (htype == kBF16 && stype == kBF16) return launch<bf16_t, bf16_t>(*a, gen, bias, blocks, vec, st);
   if (htype == kBF16 && stype == kF32) return launch<bf16_t, float>(*a, gen, bias, blocks, vec, st);
@@ -274,9 +283,10 @@ int st_block_norm_bwd(const NormArgs* a, int gen, int bias, int blocks, int htyp
   return -2;
 }
 
-// Floats of a backward's workspace (NormArgs::partial) for `arrays` column sums.
+// Floats of a backward's workspace (NormArgs::partial) for `arrays` column sums: the parts' sums, then the
+// workgroups'.
 int64_t st_block_norm_bwd_floats(int64_t rows, int width, int arrays) {
-  return (int64_t)(st_block_norm_bwd_blocks(rows, width) + kParts) * arrays * width;
+  return sum_floats(arrays, width) + (int64_t)st_block_norm_bwd_blocks(rows, width) * arrays * width;
 }
 
 // The gradients of the weights and the gate from a's partial sums.  out: dgate, dw1, db1, dw2, db2
@@ -285,9 +295,10 @@ int st_block_norm_finish(const NormArgs* a, int gen, int bias, int blocks, void*
                          int htype, hipStream_t st) {
   FinishArgs f{};
   f.arrays = (gen ? 2 : 1) * (bias ? 2 : 1);
-  float* sums = a->partial + (int64_t)blocks * f.arrays * a->width;
+  double* sums = reinterpret_cast<double*>(a->partial);
+  const float* partial = a->partial + sum_floats(f.arrays, a->width);
   const dim3 grid((unsigned)((a->width + 63) / 64), (unsigned)f.arrays, kParts);
-  block_norm_colsum_kernel<<<grid, 256, 0, st>>>(a->partial, blocks, f.arrays, a->width, sums);
+  block_norm_colsum_kernel<<<grid, 256, 0, st>>>(partial, blocks, f.arrays, a->width, sums);
   f.sums = sums;
   f.width = a->width;
   f.gen = gen;

@@ -24,15 +24,15 @@
 // more steps than the fp32 sums' way through memory costs (linear_wide_plan); a second kernel adds
 // the parts in order and runs their epilogue.
 //
-// Measured, bf16, 24576 x 4096 x 14336 (2.89 TFLOP; the library's plain products in brackets): y alone 2.33
-// ms (1.87-1.95), with bias, GELU and z 2.45-2.55, with tanh GELU, z and residual 2.63-2.77; dx 2.16-2.18
-// (2.12-2.17); dW 2.26-2.34 (2.91-2.93), of it some 16 us for the cut tiles.  8192 x 1280 x 5120: y with GELU and z 159-165
-// us (115-116 plain), dx 117-121 (102-106), dW 117 (116-124).  The chip holds its power limit here:
-// the library's kernel keeps the matrix units 86 % busy at 1.66 GHz, this one 62 % at 1.85 and 49 %
-// (epilogues) at 2.1, with no LDS conflicts and 16 % of the time in waits.  Lost to this schedule: both
-// regions released at MFMA 40 and publication at 96 (1-3 % slower), copies three MFMAs apart (6 %),
-// other row groups (0-4 %), staggered workgroups (no change), 256 x 128 tiles with two workgroups a CU
-// (1.0 PF/s).
+// Measured, bf16, kernel times of a trace of training passes, whose operands come from memory; in brackets
+// the library's plain products in the same order.  24576 x 4096 x 14336 (2.89 TFLOP): y alone 2.36 ms (1.87),
+// with bias, GELU and z 2.65, with tanh GELU, z and residual 2.75; dx 2.17 (2.12); dW 2.33 and 0.02 for the sums
+// of its cut tiles (2.87).  8192 x 1280 x 5120: y with bias, GELU and z 188 us (123), dx 135 (123), dW 117 and 17
+// for the sums of its 100 cut tiles (141).  The chip holds its power limit here: the library's kernel keeps the
+// matrix units 84 % busy at 1.75 GHz, this one 60 % at 1.93 and 50 % (epilogues) at 2.0, with no LDS conflicts
+// and 16 % of the time in waits.  Lost to this schedule: both regions released at MFMA 40 and publication at 96
+// (1-3 % slower), copies three MFMAs apart (6 %), other row groups (0-4 %), staggered workgroups (no change),
+// 256 x 128 tiles with two workgroups a CU (1.0 PF/s).
 #pragma once
 
 #include <algorithm>
@@ -416,7 +416,8 @@ __global__ __launch_bounds__(NT, 1) void linear_wide_kernel(LinearArgs p, int gm
 
 // The parts of the cut tiles, in order, then their epilogue: an (i, j) block of a tile a workgroup.
 // Neighbouring 16 x 16 blocks of a workgroup: it then writes whole 128-byte lines.  100 tiles of two parts (52 MB)
-// take 13 us; with one block each, whose lines belong to several XCDs, 27.
+// take 17 us in a training pass; called again and again 13, and with one block each, whose lines belong to
+// several XCDs, 27.
 constexpr int kJoin = 4;
 __global__ __launch_bounds__(NT) void linear_wide_join_kernel(LinearArgs p, int gm, int nfull) {
   const int nbm = (p.M + BT - 1) / BT, nbn = (p.N + BT - 1) / BT, nv = nbm * nbn, tail = nv - nfull;

@@ -467,3 +467,31 @@ def test_strided_and_expanded_weights_beside_main_grad():
         assert torch.equal(a, b)
     w32, w16 = run(True)[4], run(False)[4]
     assert torch.equal(w32.bfloat16(), w16)  # the same sums, rounded once
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("width", [1000, 1001])
+def test_a_scalar_gate_sums_its_columns_in_64_bits(width):
+    """dgate = sum of ds h over 3001 rows: every other column adds up to 3001 (1 + 2^-20), the ones between to -3001,
+    which needs 32 bits.  A lane's own sum of three rows is exact in fp32; so is all behind it in 64 bits."""
+    h = torch.ones(3001, width, device="cuda")
+    gate = torch.ones(1, device="cuda", requires_grad=True)
+    ds = torch.full_like(h, -1.0)
+    ds[:, ::2] = 1 + 2.0 ** -20
+    _, s = ops.block_norm(h, torch.zeros_like(h), gate=gate)
+    (dg,) = torch.autograd.grad(s, gate, ds)
+    want = ds.double().sum().item()
+    assert abs(dg.item() - want) <= U32 * abs(want) * 1.01
+
+
+@pytest.mark.gpu
+def test_weight_gradients_round_once_behind_the_rows():
+    """fp32 column sums of 3001 rows: a chain of three fp32 additions a lane, the rest in 64 bits and one rounding."""
+    c = _inputs("cuda", 3001, 1001, torch.float32, gate="scalar", seed=2)
+    _, _, g = _run(c, "layer", 0.5)
+    _, _, rg = _ref(c, "layer", 0.5)
+    for k in NAMES[2:]:
+        # random signs: a term of the sums is off by some 8 roundings, a lane's chain by 3, together some 4 U of the
+        # sums' own 2-norm; 6 times that.  The gate's single sum is as large as the 2-norm of the columns' sums.
+        size = rg[k].norm().item() if k != "gate" else rg["post_weight"].norm().item() / abs(c["gate"].item())
+        assert (g[k].double().cpu() - rg[k]).norm().item() <= 6 * 4 * U32 * size, k
