@@ -16,8 +16,8 @@
 // A workgroup walks rows with a fixed stride and keeps its column sums in registers; its partial
 // sums are added up by the second kernel in a fixed order (no atomics: results repeat bit for bit).
 // Bound by HBM: h, residual (or s), dy, ds in, dh, dres out.  Measured: 24576 x 4096 bf16, both norms
-// and a channel gate, 236 us (5.1 TB/s), and 10 us for its column sums; 16384 x 1280 LayerNorm 47 + 9
-// us; 3001 x 1001 fp32 18 + 10 us.  Without the next row's loads ahead the first took 301 us.  2048
+// and a channel gate, 236-247 us (5.1-4.9 TB/s), and 10 us for its column sums; 16384 x 1280 LayerNorm
+// 46 + 9 us; 3001 x 1001 fp32 with a scalar gate 18 + 12 us.  Without the next row's loads ahead the first took 301 us.  2048
 // waves keep partial sums (512 workgroups where a wave has its own row): with half of them forward
 // and backward took 515 us instead of 373, with twice as many 391.
 #include "block_norm.h"

@@ -3,7 +3,7 @@
 // One pass over dy and z: a workgroup takes 512 columns and a run of rows, its four waves every
 // fourth row; each lane keeps its 8 columns' sums, which are folded in a fixed order and added up
 // over the runs by the second kernel (no atomics: repeatable).  db sums the unrounded dz.  Bound by
-// HBM: dy and z in, dz out: 24576 x 14336 bf16 404 us (5.2 TB/s), 8192 x 5120 50 us (5.0).
+// HBM: dy and z in, dz out: 24576 x 14336 bf16 404 us (5.2 TB/s), 8192 x 5120 53 us (4.8).
 #include <algorithm>
 
 #include "linear_act.h"

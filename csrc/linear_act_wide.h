@@ -24,10 +24,10 @@
 // more steps than the fp32 sums' way through memory costs (linear_wide_plan); a second kernel adds
 // the parts in order and runs their epilogue.
 //
-// Measured, bf16, kernel times of a trace of training passes, whose operands come from memory; in brackets
-// the library's plain products in the same order.  24576 x 4096 x 14336 (2.89 TFLOP): y alone 2.36 ms (1.87),
-// with bias, GELU and z 2.65, with tanh GELU, z and residual 2.75; dx 2.17 (2.12); dW 2.33 and 0.02 for the sums
-// of its cut tiles (2.87).  8192 x 1280 x 5120: y with bias, GELU and z 188 us (123), dx 135 (123), dW 117 and 17
+// Measured, bf16, kernel times of a trace of training passes, whose operands come from memory (ranges: cards
+// differ by up to 4 %); in brackets the library's plain products in the same order.  24576 x 4096 x 14336 (2.89 TFLOP): y alone 2.36 ms (1.87),
+// with bias, GELU and z 2.65, with tanh GELU, z and residual 2.75-2.79; dx 2.17-2.22 (2.12); dW 2.33-2.38 and 0.02
+// for the sums of its cut tiles (2.87).  8192 x 1280 x 5120: y with bias, GELU and z 188 us (123), dx 135 (123), dW 117 and 17
 // for the sums of its 100 cut tiles (141).  The chip holds its power limit here: the library's kernel keeps the
 // matrix units 84 % busy at 1.75 GHz, this one 60 % at 1.93 and 50 % (epilogues) at 2.0, with no LDS conflicts
 // and 16 % of the time in waits.  Lost to this schedule: both regions released at MFMA 40 and publication at 96
